@@ -38,7 +38,7 @@
 extern "C" {
 #endif
 
-#define B200_ABI_VERSION 13
+#define B200_ABI_VERSION 14
 
 #define B200_DTYPE_F32 0
 #define B200_DTYPE_BF16 1
@@ -802,6 +802,55 @@ int b200_sigmoid_decode(const void* q, const void* k_cache, const void* v_cache,
 int b200_moe_softmax_route(const float* logits, const float* bias, int32_t num_tokens, int32_t num_experts, int32_t top,
                            int32_t* sorted_token, float* weight, int32_t* expert_offsets, int32_t* slot_to_row, void* workspace,
                            size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * Several answers to a prompt and contexts beyond the cache: attention over a sliding window and the first tokens, filtered
+ * sampling, pages that are copied and compacted (the reference has no counterpart).
+ * ------------------------------------------------------------------------------------------- */
+
+/* Attention over the paged pools for ragged portions: query i of a sequence, at position p = k_len - q_len + i, sees the keys j
+ * with 0 <= p - j and (p - j < window or j < first); window >= 1, first >= 0.  Rows that see no key become zeros; rows of out
+ * behind the last sequence stay as they are.  Rows of the pools and table entries that no query sees are not used: pages between
+ * the first tokens and the window may have been given back (any entry).  A visible key on a page outside the pool is left out and
+ * reported.  q [total_q, Hq, D] with a token stride in elements; pools [num_blocks, block_size, Hkv, D | Dv]; out
+ * [total_q, Hq, Dv]; block_tables [num_seqs, bt_width] with a row stride.  Head sizes up to 1024. */
+int b200_window_attention(const void* q, int64_t q_token_stride, const void* k_cache, const void* v_cache, void* out,
+                          int64_t total_q, const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k, int32_t num_seqs,
+                          int32_t max_seqlen_q, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim_qk,
+                          int32_t head_dim_v, float scale, const int32_t* block_tables, int64_t bt_stride, int32_t bt_width,
+                          int32_t block_size, int64_t num_blocks, int32_t window, int32_t first, int32_t dtype, int32_t* status, void* stream);
+
+/* The same for one token per sequence, at position context_lens[i] - 1.  q and out are contiguous. */
+int b200_window_decode(const void* q, const void* k_cache, const void* v_cache, void* out, const int32_t* block_tables,
+                       int64_t bt_stride, int32_t bt_width, const int64_t* context_lens, int32_t batch, int32_t num_q_heads,
+                       int32_t num_kv_heads, int32_t head_dim_qk, int32_t head_dim_v, int32_t block_size, int64_t num_blocks, float scale,
+                       int32_t window, int32_t first, int32_t dtype, int32_t* status, void* stream);
+
+/* One token per row of logits under filters of the row's own, drawn with uniforms[row] in [0, 1).  Tokens are ordered by logit,
+ * equal ones by number; w_i = exp((x_i - max x) / T).  top_k (<= 0 or >= vocab: off) keeps the first k; top_p (>= 1: off) of those
+ * the shortest run from the front whose weights reach top_p of their sum, at least one token; min_p (<= 0: off, at most 1) of
+ * those the ones with w_i >= min_p; the draw is the first kept token, by number, at which the running sum of kept weights exceeds
+ * u times their sum.  T <= 0 and rows without a logit above -inf: the first of the highest logits.  NaN counts as -inf.  The filter
+ * arrays may be NULL (off).  vocab_size <= 2^24. */
+int b200_sample_filtered(const void* logits, int64_t row_stride, int64_t num_rows, int32_t vocab_size, const float* uniforms,
+                         const float* temperatures, const int32_t* top_k, const float* top_p, const float* min_p,
+                         int64_t* out_tokens, int32_t dtype, void* stream);
+
+/* Pools that share page ids: pools [num_pools] holds their device addresses and page_bytes their bytes per page (device arrays).
+ * Page target[j] of every pool becomes page source[j]; pairs with a negative id are left out, ids outside the pool reported.  A pair
+ * whose target is also a source of the call or the target of an earlier pair is not carried out and reported (B200_ERR_ARG). */
+size_t b200_copy_pages_workspace_bytes(int32_t num_pairs);
+int b200_copy_pages(const int64_t* pools, const int64_t* page_bytes, int32_t num_pools, int64_t num_pages, const int32_t* source,
+                    const int32_t* target, int32_t num_pairs, void* workspace, size_t workspace_bytes, int32_t* status,
+                    void* stream);
+
+/* Moves the pages that block_tables [rows, width] names (negative entries name none) to the front of all pools: with L of them, those
+ * with an id >= L go, in ascending order, to the unnamed ids < L, in ascending order; nothing else is written in the pools.
+ * out_tables [rows, width] = the tables with the new ids, page_map [num_pages] = new id or -1, counts = {L, moves}; source and target
+ * [num_pages] receive the moves.  Entries outside the pool are reported and become -1. */
+int b200_compact_pages(const int64_t* pools, const int64_t* page_bytes, int32_t num_pools, int64_t num_pages,
+                       const int32_t* block_tables, int64_t bt_stride, int64_t rows, int32_t width, int32_t* out_tables,
+                       int32_t* page_map, int32_t* source, int32_t* target, int32_t* counts, int32_t* status, void* stream);
 
 /* ---------------------------------------------------------------------------------------------
  * Diagnostic (no counterpart in the reference, which has no device code): runs the give-up path of the

@@ -1,0 +1,213 @@
+// Pages of a paged cache: copies (forks, moves) and compaction.
+//
+// A cache is a set of pools, one per layer and kind of row, that share page ids: page i of every pool belongs to the same tokens.
+// Copy: page target[j] of every pool becomes page source[j]; pairs with a negative id are left out.  The copies of a call run in no order, so
+// a pair whose target is also a source of the call, or the target of an earlier pair, is not carried out and reported: every CTA looks
+// through the pairs for its own one's, or, beyond kLookedThrough of them, a kernel in front does it once.
+// Compaction: with L pages in use (named in a block table), the pages in use from id L on move, in ascending order, to the unused ids
+// below L, in ascending order.  What moves is never a target and the old places keep their contents, so all copies may run at once.
+#include "common.cuh"
+
+namespace b200 {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kLookedThrough = 1024;
+
+struct CopyArgs {
+  const int64_t* pools;      // [num_pools] addresses
+  const int64_t* bytes;      // [num_pools] bytes of a page
+  const int32_t* source;
+  const int32_t* target;
+  const int32_t* count;      // pairs, or null: all
+  int n, num_pools;
+  bool look;                 // for conflicts
+  int64_t num_pages;
+  int32_t* status;
+};
+
+__device__ __forceinline__ bool in_pool(int id, int64_t num_pages) {
+  return static_cast<uint64_t>(static_cast<int64_t>(id)) < static_cast<uint64_t>(num_pages);
+}
+
+// Pair j against the pairs lo, lo + step, ... below hi.
+__device__ __forceinline__ bool conflicts(int to, int j, const int32_t* source, const int32_t* target, int base, int lo, int hi, int step) {
+  bool bad = false;
+  for (int i = lo; i < hi; i += step) {
+    const int from = source[i], other = target[i];
+    if (from < 0 || other < 0) continue;
+    bad |= (from == to && other != to) || (other == to && base + i < j);
+  }
+  return bad;
+}
+
+// checked: source, -1 for pairs that are not carried out
+__global__ void __launch_bounds__(kThreads) check_pairs_kernel(const int32_t* source, const int32_t* target, int n, int32_t* checked,
+                                                               int32_t* status) {
+  __shared__ int s_source[kThreads], s_target[kThreads];
+  const int j = blockIdx.x * kThreads + threadIdx.x;
+  const int from = j < n ? source[j] : -1, to = j < n ? target[j] : -1;
+  bool bad = false;
+  for (int base = 0; base < n; base += kThreads) {
+    __syncthreads();
+    const int i = base + threadIdx.x;
+    s_source[threadIdx.x] = i < n ? source[i] : -1;
+    s_target[threadIdx.x] = i < n ? target[i] : -1;
+    __syncthreads();
+    bad |= conflicts(to, j, s_source, s_target, base, 0, kThreads, 1);
+  }
+  if (j >= n) return;
+  bad = bad && from >= 0 && to >= 0 && from != to;
+  if (bad) report(status, B200_ERR_ARG);
+  checked[j] = bad ? -1 : from;
+}
+
+__global__ void __launch_bounds__(kThreads) copy_pages_kernel(const CopyArgs a) {
+  const int pool = blockIdx.y, n = a.count ? min(*a.count, a.n) : a.n;
+  const int64_t bytes = a.bytes[pool];
+  uint8_t* base = reinterpret_cast<uint8_t*>(a.pools[pool]);
+  const bool wide = (reinterpret_cast<uintptr_t>(base) | static_cast<uintptr_t>(bytes)) % 16 == 0;
+  for (int j = blockIdx.x; j < n; j += gridDim.x) {
+    const int from = a.source[j], to = a.target[j];
+    if (from < 0 || to < 0 || from == to) continue;
+    if (a.look && __syncthreads_or(conflicts(to, j, a.source, a.target, 0, threadIdx.x, n, kThreads))) {
+      if (threadIdx.x == 0) report(a.status, B200_ERR_ARG);
+      continue;
+    }
+    if (!in_pool(from, a.num_pages) || !in_pool(to, a.num_pages)) {
+      if (threadIdx.x == 0) report(a.status, B200_ERR_BOUNDS);
+      continue;
+    }
+    const uint8_t* src = base + from * bytes;
+    uint8_t* dst = base + to * bytes;
+    if (wide) {
+      for (int64_t i = threadIdx.x * 16; i < bytes; i += kThreads * 16)
+        *reinterpret_cast<uint4*>(dst + i) = *reinterpret_cast<const uint4*>(src + i);
+    } else {
+      for (int64_t i = threadIdx.x; i < bytes; i += kThreads) dst[i] = src[i];
+    }
+  }
+}
+
+// page_map (zeros before): 1 for the pages in use
+__global__ void __launch_bounds__(kThreads) mark_pages_kernel(const int32_t* tables, int64_t row_stride, int64_t rows, int width,
+                                                              int64_t num_pages, int32_t* page_map, int32_t* status) {
+  const int64_t total = rows * width;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; i < total; i += static_cast<int64_t>(gridDim.x) * kThreads) {
+    const int id = tables[i / width * row_stride + i % width];
+    if (in_pool(id, num_pages)) page_map[id] = 1;
+    else if (id >= 0) report(status, B200_ERR_BOUNDS);
+  }
+}
+
+constexpr int kPlanThreads = 1024;
+
+// Inclusive sum over the CTA.
+__device__ __forceinline__ int block_sum_upto(int v, int* s_warp, int* total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += y;
+  }
+  __syncthreads();
+  if (lane == 31) s_warp[warp] = v;
+  __syncthreads();
+  int before = 0, all = 0;
+  for (int w = 0; w < kPlanThreads / 32; ++w) {
+    before += w < warp ? s_warp[w] : 0;
+    all += s_warp[w];
+  }
+  *total = all;
+  return v + before;
+}
+
+// page_map: marks -> new ids (-1: unused); source / target: the moves; counts: pages in use, moves.  One CTA, a run of pages per thread.
+__global__ void __launch_bounds__(kPlanThreads) plan_pages_kernel(int32_t* page_map, int num_pages, int32_t* source, int32_t* target,
+                                                                  int32_t* counts) {
+  __shared__ int s_warp[kPlanThreads / 32];
+  const int per = (num_pages + kPlanThreads - 1) / kPlanThreads;
+  const int lo = min(static_cast<int64_t>(threadIdx.x) * per, static_cast<int64_t>(num_pages)), hi = min(lo + per, num_pages);
+  int mine = 0, live, moves;
+  for (int i = lo; i < hi; ++i) mine += page_map[i];
+  block_sum_upto(mine, s_warp, &live);
+  int holes = 0, movers = 0;
+  for (int i = lo; i < hi; ++i) (i < live ? holes : movers) += i < live ? !page_map[i] : page_map[i];
+  int hole = block_sum_upto(holes, s_warp, &moves) - holes, mover = block_sum_upto(movers, s_warp, &moves) - movers;
+  for (int i = lo; i < hi; ++i) {
+    const bool used = page_map[i];
+    if (i < live && !used) target[hole++] = i;
+    if (i >= live && used) source[mover++] = i;
+    page_map[i] = used && i < live ? i : -1;
+  }
+  __syncthreads();
+  for (int j = threadIdx.x; j < moves; j += kPlanThreads) page_map[source[j]] = target[j];
+  if (threadIdx.x == 0) counts[0] = live, counts[1] = moves;
+}
+
+__global__ void __launch_bounds__(kThreads) rename_pages_kernel(const int32_t* tables, int64_t row_stride, int64_t rows, int width,
+                                                                int64_t num_pages, const int32_t* page_map, int32_t* out) {
+  const int64_t total = rows * width;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; i < total; i += static_cast<int64_t>(gridDim.x) * kThreads) {
+    const int id = tables[i / width * row_stride + i % width];
+    out[i] = in_pool(id, num_pages) ? page_map[id] : -1;
+  }
+}
+
+int grid_for(int64_t items) {
+  const int64_t ctas = (items + kThreads - 1) / kThreads;
+  return static_cast<int>(ctas < 1184 ? ctas : 1184);
+}
+
+int copy(const CopyArgs& a, cudaStream_t s) {
+  if (a.n == 0 || a.num_pools == 0) return B200_OK;
+  if (a.num_pools > 65535) return B200_ERR_TOO_LARGE;
+  const int wanted = 4736 / a.num_pools + 1;
+  copy_pages_kernel<<<dim3(a.n < wanted ? a.n : wanted, a.num_pools), kThreads, 0, s>>>(a);
+  return launch_result();
+}
+
+}  // namespace
+}  // namespace b200
+
+extern "C" size_t b200_copy_pages_workspace_bytes(int32_t num_pairs) {
+  return num_pairs > b200::kLookedThrough ? static_cast<size_t>(num_pairs) * sizeof(int32_t) : 0;
+}
+
+extern "C" int b200_copy_pages(const int64_t* pools, const int64_t* page_bytes, int32_t num_pools, int64_t num_pages,
+                               const int32_t* source, const int32_t* target, int32_t num_pairs, void* workspace,
+                               size_t workspace_bytes, int32_t* status, void* stream) {
+  using namespace b200;
+  if (num_pools < 0 || num_pages < 0 || num_pairs < 0) return B200_ERR_ARG;
+  if (num_pairs == 0 || num_pools == 0) return B200_OK;
+  if (!pools || !page_bytes || !source || !target) return B200_ERR_ARG;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  CopyArgs a{pools, page_bytes, source, target, nullptr, num_pairs, num_pools, num_pairs <= kLookedThrough, num_pages, status};
+  if (!a.look) {
+    if (!workspace || workspace_bytes < b200_copy_pages_workspace_bytes(num_pairs)) return B200_ERR_WORKSPACE;
+    int32_t* checked = static_cast<int32_t*>(workspace);
+    check_pairs_kernel<<<(num_pairs - 1) / kThreads + 1, kThreads, 0, s>>>(source, target, num_pairs, checked, status);
+    a.source = checked;
+  }
+  return copy(a, s);
+}
+
+extern "C" int b200_compact_pages(const int64_t* pools, const int64_t* page_bytes, int32_t num_pools, int64_t num_pages,
+                                  const int32_t* block_tables, int64_t bt_stride, int64_t rows, int32_t width, int32_t* out_tables,
+                                  int32_t* page_map, int32_t* source, int32_t* target, int32_t* counts, int32_t* status, void* stream) {
+  using namespace b200;
+  if (num_pools < 0 || num_pages < 0 || rows < 0 || width < 0 || bt_stride < width) return B200_ERR_ARG;
+  if (num_pages > 2147483647) return B200_ERR_TOO_LARGE;
+  if (!counts || (num_pages > 0 && (!page_map || !source || !target)) || (rows * width > 0 && (!block_tables || !out_tables)) ||
+      (num_pools > 0 && (!pools || !page_bytes)))
+    return B200_ERR_ARG;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (num_pages > 0 && cudaMemsetAsync(page_map, 0, num_pages * sizeof(int32_t), s) != cudaSuccess) return launch_result(cudaErrorUnknown);
+  const int64_t entries = rows * width;
+  if (entries > 0) mark_pages_kernel<<<grid_for(entries), kThreads, 0, s>>>(block_tables, bt_stride, rows, width, num_pages, page_map, status);
+  plan_pages_kernel<<<1, kPlanThreads, 0, s>>>(page_map, static_cast<int>(num_pages), source, target, counts);
+  if (entries > 0) rename_pages_kernel<<<grid_for(entries), kThreads, 0, s>>>(block_tables, bt_stride, rows, width, num_pages, page_map, out_tables);
+  const int rc = launch_result();
+  if (rc != B200_OK || num_pages == 0) return rc;
+  return copy({pools, page_bytes, source, target, counts + 1, static_cast<int>(num_pages), num_pools, false, num_pages, status}, s);
+}

@@ -1609,3 +1609,196 @@ def moe_softmax_route(logits: torch.Tensor, bias: torch.Tensor, top: int):
     check(lib.b200_moe_softmax_route(logits.data_ptr(), bias.data_ptr(), T, E, int(top), tok.data_ptr(), w.data_ptr(),
                                      offs.data_ptr(), slot.data_ptr(), ws.data_ptr(), ws.numel(), _stream()), "moe_softmax_route")
     return tok, w, offs, slot
+
+
+# ------------------------------------------------------------------------------------------------
+# a window and the first tokens, filtered sampling, pages of a cache
+# ------------------------------------------------------------------------------------------------
+def _on_current(dev: torch.device) -> None:
+    """Launches go to the current device's stream."""
+    if dev.index != torch._C._cuda_getDevice():
+        raise ValueError(f"the tensors are on {dev}, which is not the current device")
+
+
+def _window_args(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor, num_seqs: int, window: int,
+                 first: int, out: torch.Tensor | None) -> torch.Tensor:
+    """Checks what both forms of the attention share; returns the output tensor."""
+    if q.dim() != 3 or k_cache.dim() != 4 or v_cache.dim() != 4:
+        raise ValueError("q must be [tokens, Hq, D] and the caches [num_blocks, block_size, Hkv, D]")
+    T, Hq, D = q.shape
+    Hkv, Dv = k_cache.shape[2], v_cache.shape[3]
+    if k_cache.shape[3] != D or v_cache.shape[:3] != k_cache.shape[:3] or k_cache.dtype != q.dtype or v_cache.dtype != q.dtype:
+        raise ValueError("cache shape/dtype does not match q")
+    if Hkv == 0 or Hq % Hkv:
+        raise ValueError("the query heads must be a multiple of the key heads")
+    if not (k_cache.is_contiguous() and v_cache.is_contiguous()):
+        raise ValueError("caches must be contiguous")
+    if block_tables.dtype != torch.int32 or block_tables.dim() != 2 or block_tables.shape[0] != num_seqs \
+            or (block_tables.shape[1] != 1 and block_tables.stride(1) != 1):
+        raise ValueError("block_tables must be int32 [num_seqs, maxb] with contiguous rows")
+    if num_seqs and block_tables.shape[1] == 0:
+        raise ValueError("block_tables must have a column")
+    if not 1 <= window <= 0x7FFFFFFF or not 0 <= first <= 0x7FFFFFFF:
+        raise ValueError("window must be at least 1 and first at least 0")
+    if out is None:
+        return torch.empty((T, Hq, Dv), dtype=q.dtype, device=q.device)
+    if out.shape != (T, Hq, Dv) or out.dtype != q.dtype or not out.is_contiguous():
+        raise ValueError("out must be a contiguous [tokens, Hq, Dv] tensor of q's dtype")
+    return out
+
+
+def window_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor, cu_seqlens_q: torch.Tensor,
+                     cu_seqlens_k: torch.Tensor, max_seqlen_q: int, scale: float, window: int, first: int = 0,
+                     out: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of ragged portions over a paged cache, which already holds their own keys and values: the query at position p sees key j
+    when 0 <= p - j and (p - j < window or j < first) (``b200_window_attention``).
+
+    q: [tokens, Hq, D], token stride free, portions at the ends of contexts of ``cu_seqlens_k`` lengths; caches
+    [num_blocks, block_size, Hkv, D] (value heads may have a size of their own); ``block_tables`` [num_seqs, maxb] int32, of which only
+    the entries of pages with a visible key count.  Rows that see no key are zeros; rows behind the last sequence are left as they
+    are (``out``).  Returns [tokens, Hq, Dv]."""
+    dev = _cuda(q, k_cache, v_cache, block_tables, cu_seqlens_q, cu_seqlens_k, out)
+    _on_current(dev)
+    for cu in (cu_seqlens_q, cu_seqlens_k):
+        if cu.dtype != torch.int32 or cu.dim() != 1 or not cu.is_contiguous() or cu.numel() != cu_seqlens_q.numel() or cu.numel() == 0:
+            raise ValueError("cu_seqlens must be contiguous int32 tensors of num_seqs + 1 entries")
+    num_seqs = cu_seqlens_q.numel() - 1
+    out = _window_args(q, k_cache, v_cache, block_tables, num_seqs, window, first, out)
+    T, Hq, D = q.shape
+    nb, bs, Hkv, Dv = v_cache.shape
+    if T and (q.stride(2) != 1 or (Hq > 1 and q.stride(1) != D)):
+        raise ValueError("q heads must be contiguous")
+    if max_seqlen_q < 0:
+        raise ValueError("max_seqlen_q must not be negative")
+    check(lib.b200_window_attention(q.data_ptr(), q.stride(0), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), T,
+                                    cu_seqlens_q.data_ptr(), cu_seqlens_k.data_ptr(), num_seqs, min(int(max_seqlen_q), T), Hq, Hkv, D, Dv,
+                                    float(scale), block_tables.data_ptr(), block_tables.stride(0), block_tables.shape[1], bs, nb, int(window),
+                                    int(first),
+                                    _dt(q), status_word(dev).data_ptr(), _stream()), "window_attention")
+    return out
+
+
+def window_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor, context_lens: torch.Tensor,
+                  scale: float, window: int, first: int = 0, out: torch.Tensor | None = None) -> torch.Tensor:
+    """``window_attention`` for one token per sequence, the last of ``context_lens`` [B] int64 tokens (``b200_window_decode``).
+    q: [B, Hq, D] contiguous.  Returns [B, Hq, Dv]; zeros for contexts without tokens."""
+    dev = _cuda(q, k_cache, v_cache, block_tables, context_lens, out)
+    _on_current(dev)
+    out = _window_args(q, k_cache, v_cache, block_tables, q.shape[0], window, first, out)
+    B, Hq, D = q.shape
+    nb, bs, Hkv, Dv = v_cache.shape
+    if context_lens.dtype != torch.int64 or context_lens.shape != (B,) or not context_lens.is_contiguous():
+        raise ValueError("context_lens must be a contiguous int64 [B] tensor")
+    if not q.is_contiguous():
+        raise ValueError("q must be contiguous")
+    check(lib.b200_window_decode(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), block_tables.data_ptr(),
+                                 block_tables.stride(0), block_tables.shape[1], context_lens.data_ptr(), B, Hq, Hkv, D, Dv, bs, nb, float(scale),
+                                 int(window), int(first), _dt(q), status_word(dev).data_ptr(), _stream()), "window_decode")
+    return out
+
+
+def sample_filtered(logits: torch.Tensor, uniforms: torch.Tensor, temperatures: torch.Tensor, top_k: torch.Tensor | None = None,
+                    top_p: torch.Tensor | None = None, min_p: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """One token per row of ``logits`` [B, V] under temperature, top-k, top-p and min-p, drawn with ``uniforms`` [B] in [0, 1)
+    (``b200_sample_filtered``).  Filters are per row: ``top_k`` int32 (<= 0 or >= V: off), ``top_p`` fp32 (>= 1: off), ``min_p`` fp32
+    (<= 0: off), None for all rows off; rows with a temperature <= 0 are greedy.  Equal logits count in the order of their tokens, and the
+    draw is the same for every launch: the same row and random number always give the same token.  Returns int64 [B]."""
+    dev = _cuda(logits, uniforms, temperatures, top_k, top_p, min_p, out)
+    _on_current(dev)
+    if logits.dim() != 2 or logits.shape[1] == 0:
+        raise ValueError("logits must be [B, V]")
+    B, V = logits.shape
+    if V > 1 and logits.stride(1) != 1:
+        raise ValueError("logits rows must be contiguous")
+    if B > 1 and logits.stride(0) < V:
+        raise ValueError("logits rows must not overlap")
+    for name, t in (("uniforms", uniforms), ("temperatures", temperatures), ("top_p", top_p), ("min_p", min_p)):
+        _f32vec(name, t, B)
+    if top_k is not None and (top_k.dtype != torch.int32 or top_k.numel() != B or not top_k.is_contiguous()):
+        raise ValueError("top_k must be contiguous int32 [B]")
+    if out is None:
+        out = torch.empty(B, dtype=torch.int64, device=logits.device)
+    elif out.dtype != torch.int64 or out.numel() != B or not out.is_contiguous():
+        raise ValueError("out must be contiguous int64 [B]")
+    check(lib.b200_sample_filtered(logits.data_ptr(), logits.stride(0) if B > 1 else V, B, V, uniforms.data_ptr(), temperatures.data_ptr(),
+                                   _ptr(top_k), _ptr(top_p), _ptr(min_p), out.data_ptr(), _dt(logits), _stream()), "sample_filtered")
+    return out
+
+
+class PagePools:
+    """Pools of one cache, made once: contiguous tensors [num_pages, ...] on one device that share page ids (``copy_pages``,
+    ``compact_pages``)."""
+
+    def __init__(self, pools):
+        self.tensors = [pools] if isinstance(pools, torch.Tensor) else list(pools)
+        if not self.tensors:
+            raise ValueError("a cache has a pool at least")
+        self.device = _cuda(*self.tensors)
+        self.num_pages = self.tensors[0].shape[0] if self.tensors[0].dim() else 0
+        for t in self.tensors:
+            if t.dim() < 1 or t.shape[0] != self.num_pages or not t.is_contiguous():
+                raise ValueError("pools must be contiguous tensors with the same number of pages")
+        if self.num_pages > 0x7FFFFFFF:
+            raise ValueError("at most 2^31 - 1 pages")
+        size = lambda t: t.numel() * t.element_size()
+        spans = sorted((t.data_ptr(), size(t)) for t in self.tensors if t.numel())
+        if any(a + n > b for (a, n), (b, _) in zip(spans, spans[1:])):
+            raise ValueError("pools must not overlap")
+        addresses = [t.data_ptr() for t in self.tensors]
+        page_bytes = [size(t) // self.num_pages if self.num_pages else 0 for t in self.tensors]
+        self._table = torch.tensor([addresses, page_bytes], dtype=torch.int64).to(self.device)
+
+    def _pointers(self):
+        return self._table[0].data_ptr(), self._table[1].data_ptr(), len(self.tensors), self.num_pages
+
+
+def _page_ids(name: str, t: torch.Tensor) -> None:
+    if t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous int32 vector")
+
+
+def copy_pages(pools: PagePools, source: torch.Tensor, target: torch.Tensor) -> None:
+    """Page ``target[j]`` of every pool becomes page ``source[j]`` (int32 on the device; pairs with a negative id are left out): forks
+    of the page that sequences go on writing, moves (``b200_copy_pages``).  A source may be copied several times; a pair whose target is
+    also a source of the call or the target of an earlier pair is not carried out, and the next ``check_status`` raises, as for ids
+    outside the pools."""
+    dev = _cuda(pools.tensors[0], source, target)
+    _on_current(dev)
+    _page_ids("source", source)
+    _page_ids("target", target)
+    if source.numel() != target.numel():
+        raise ValueError("source and target must have the same length")
+    n = source.numel()
+    nbytes = lib.b200_copy_pages_workspace_bytes(n)
+    scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    check(lib.b200_copy_pages(*pools._pointers(), source.data_ptr(), target.data_ptr(), n, _ptr(scratch), nbytes,
+                              status_word(dev).data_ptr(), _stream()), "copy_pages")
+
+
+@dataclass
+class CompactedPages:
+    block_tables: torch.Tensor   # [rows, width] int32: the tables with the new page ids
+    page_map: torch.Tensor       # [num_pages] int32: new id of a page, -1 where no table names it
+    counts: torch.Tensor         # [2] int32: pages in use, pages moved
+
+
+def compact_pages(pools: PagePools, block_tables: torch.Tensor) -> CompactedPages:
+    """Moves the pages that ``block_tables`` [rows, width] int32 names (negative entries name none; several entries may name one) to the
+    front of all pools (``b200_compact_pages``): with L of them, those from id L on go, in ascending order, to the free ids below L, in
+    ascending order.  The tables given are left as they are and the moved pages' old places keep their contents; no host wait.  Sequences
+    go on with the tables returned."""
+    dev = _cuda(pools.tensors[0], block_tables)
+    _on_current(dev)
+    if block_tables.dtype != torch.int32 or block_tables.dim() != 2 or (block_tables.shape[1] > 1 and block_tables.stride(1) != 1):
+        raise ValueError("block_tables must be int32 [rows, width] with contiguous rows")
+    rows, width = block_tables.shape
+    stride = block_tables.stride(0) if rows > 1 else width
+    if stride < width:
+        raise ValueError("block_tables rows must not overlap")
+    tables = torch.empty((rows, width), dtype=torch.int32, device=dev)
+    page_map, source, target = (torch.empty(pools.num_pages, dtype=torch.int32, device=dev) for _ in range(3))
+    counts = torch.empty(2, dtype=torch.int32, device=dev)
+    check(lib.b200_compact_pages(*pools._pointers(), block_tables.data_ptr(), stride, rows, width, tables.data_ptr(), page_map.data_ptr(),
+                                 source.data_ptr(), target.data_ptr(), counts.data_ptr(), status_word(dev).data_ptr(), _stream()),
+          "compact_pages")
+    return CompactedPages(tables, page_map, counts)
