@@ -11,9 +11,13 @@
 // Measured at 64 sequences of 64 to 1024 tokens, 16/4 heads x 64: 28 us (the general kernel, a CTA per sequence and query
 // head: 307 us); 128 sequences of 2048 tokens, 32/8 x 128: 346 us, 6.2 TB/s.  With the table read inside the trips and a full
 // reduction of every score the latter took 457 us.
+//
+// WINDOW: a token sees the last `window` tokens of its context and its first ones (window_attention.cu).  The visible tokens are numbered
+// through, first tokens first, and what follows cuts and walks these numbers; a share with tokens of both parts is walked in two.
 #include <cooperative_groups.h>
 
 #include "sequences.cuh"
+#include "window_attention.cuh"
 
 namespace b200 {
 namespace {
@@ -33,6 +37,8 @@ struct DecodeF32Args {
   float scale_log2;
   const float* sink;         // [Hq] or null
   int32_t* status;
+  int window, first;         // WINDOW kernels
+  int bt_width;              // WINDOW kernels: entries of a table row
 };
 
 constexpr int kWarps = 4, kThreads = kWarps * 32;
@@ -42,7 +48,7 @@ constexpr int kTable = 1024; // block numbers held at a time
 constexpr size_t kRingBytes = static_cast<size_t>(kWarps) * kStages * kUnroll * 4 * 32 * sizeof(float4);
 
 // GC: query heads of the CTA
-template <int D, int GC>
+template <int D, int GC, bool WINDOW>
 __global__ void __launch_bounds__(kThreads, 3) decode_f32_kernel(const DecodeF32Args a) {
   constexpr int LP = D / 8;                    // lanes of a token
   constexpr int TW = 32 / LP;                  // tokens of a warp
@@ -57,12 +63,15 @@ __global__ void __launch_bounds__(kThreads, 3) decode_f32_kernel(const DecodeF32
   const int seq = blockIdx.z, head0 = blockIdx.y * GC, kvh = head0 / (a.Hq / a.Hkv);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, sub = lane % LP, grp = lane / LP;
   int64_t len64 = a.lens[seq];
-  const int64_t cap = a.bt_stride * a.bs;
+  const int64_t cap = (WINDOW ? a.bt_width : a.bt_stride) * a.bs;
   if (len64 > cap) {
     if (tid == 0) report(a.status, B200_ERR_BOUNDS);
     len64 = cap;
   }
-  const int len = len64 > 0 ? static_cast<int>(len64) : 0;
+  const int context = len64 > 0 ? static_cast<int>(len64) : 0;
+  // visible tokens: the first `front`, then those behind `gap` more
+  const int front = WINDOW ? min(a.first, max(context - a.window, 0)) : 0, gap = WINDOW ? max(context - a.window, 0) - front : 0;
+  const int len = context - gap;
   const int32_t* table = a.bt + static_cast<int64_t>(seq) * a.bt_stride;
 
   // lane `sub` of a token ends up with the scores of the pairs own, own + 1, ... of a trip
@@ -95,8 +104,9 @@ __global__ void __launch_bounds__(kThreads, 3) decode_f32_kernel(const DecodeF32
   auto page_of = [&](int t) { return shift >= 0 ? t >> shift : t / a.bs; };
   float4* slots = ring + (warp * kStages * kUnroll * 4) * 32 + lane;
   const int span = static_cast<int>(min(static_cast<int64_t>(kTable - 1) * a.bs, static_cast<int64_t>(len)));
-  for (int base = lo; base < hi; base += span) {
-    const int end = min(base + span, hi), page0 = page_of(base), pages = page_of(end - 1) - page0 + 1;
+  auto walk = [&](const int from, const int to) {
+  for (int base = from; base < to; base += span) {
+    const int end = min(base + span, to), page0 = page_of(base), pages = page_of(end - 1) - page0 + 1;
     __syncthreads();
     for (int i = tid; i < pages; i += kThreads) {
       int id = table[page0 + i];
@@ -230,6 +240,9 @@ __global__ void __launch_bounds__(kThreads, 3) decode_f32_kernel(const DecodeF32
     }
     cp_async_wait<0>();
   }
+  };
+  if (WINDOW && lo < front) walk(lo, min(hi, front));
+  walk(WINDOW ? max(lo, front) + gap : lo, hi + gap);
   // ---- lane groups of the warp, warps of the CTA, CTAs of the cluster ----
 #pragma unroll
   for (int g = 0; g < GC; ++g) {
@@ -294,13 +307,13 @@ __global__ void __launch_bounds__(kThreads, 3) decode_f32_kernel(const DecodeF32
   if (used > 1) cluster.sync();            // nobody leaves while another CTA reads its shared memory
 }
 
-template <int D, int GC>
+template <int D, int GC, bool WINDOW>
 int launch_heads(const DecodeF32Args& a, int batch, int ranks, cudaStream_t s) {
   static bool configured[64] = {false};       // racing threads set the same attribute
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev >= 0 && dev < 64 && !configured[dev]) {
-    if (cudaFuncSetAttribute(decode_f32_kernel<D, GC>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    if (cudaFuncSetAttribute(decode_f32_kernel<D, GC, WINDOW>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                              static_cast<int>(kRingBytes)) != cudaSuccess)
       return B200_ERR_LAUNCH;
     configured[dev] = true;
@@ -316,10 +329,10 @@ int launch_heads(const DecodeF32Args& a, int batch, int ranks, cudaStream_t s) {
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return launch_result(cudaLaunchKernelEx(&cfg, decode_f32_kernel<D, GC>, a));
+  return launch_result(cudaLaunchKernelEx(&cfg, decode_f32_kernel<D, GC, WINDOW>, a));
 }
 
-template <int D>
+template <int D, bool WINDOW = false>
 int launch_dim(const DecodeF32Args& a, int batch, cudaStream_t s) {
   int sms = sm_count_cached();
   if (sms <= 0) sms = 148;
@@ -328,7 +341,8 @@ int launch_dim(const DecodeF32Args& a, int batch, cudaStream_t s) {
   // which evens out batches of unequal contexts.  Three CTAs fit an SM at head sizes 32 and 64, two at 128, so four are more than one
   // round; the line is where the times lie, not a wave (one, two, four, eight CTAs per context, 64 .. 1,024 tokens: 64 sequences at 16/4 x
   // 64 19.5, 17.0, 19.2, 25.8 us, 32 at 32/8 x 128 34, 32, 38, 52; 128 .. 8,192 tokens, 64 at 16/4 x 64 129, 75, 64, 65).
-  const int64_t pairs = static_cast<int64_t>(batch) * (a.Hq / GC), keys = a.bt_stride * a.bs;
+  const int64_t pairs = static_cast<int64_t>(batch) * (a.Hq / GC), seen = static_cast<int64_t>(a.window) + a.first;
+  const int64_t table = (WINDOW ? a.bt_width : a.bt_stride) * a.bs, keys = WINDOW && seen < table ? seen : table;
   // The general kernel keeps contexts of up to eight tokens, where the merges are the call (one token at 16/4 x 64: 4.7 against 2.8 us), and
   // large batches of up to sixteen where no heads share the rows (256 x 16 at 16/16 x 32: 28 against 19).
   if (keys <= 8 || (keys <= 16 && GC == 1 && pairs >= 2048)) return B200_ERR_UNSUPPORTED;
@@ -337,9 +351,9 @@ int launch_dim(const DecodeF32Args& a, int batch, cudaStream_t s) {
   while (ranks < 8 && static_cast<int64_t>(ranks) * trip < keys &&
          pairs * ranks * 2 <= (keys / ranks > 1024 ? 8 : 4) * static_cast<int64_t>(sms))
     ranks *= 2;
-  if (GC == 4) return launch_heads<D, 4>(a, batch, ranks, s);
-  if (GC == 2) return launch_heads<D, 2>(a, batch, ranks, s);
-  return launch_heads<D, 1>(a, batch, ranks, s);
+  if (GC == 4) return launch_heads<D, 4, WINDOW>(a, batch, ranks, s);
+  if (GC == 2) return launch_heads<D, 2, WINDOW>(a, batch, ranks, s);
+  return launch_heads<D, 1, WINDOW>(a, batch, ranks, s);
 }
 
 }  // namespace
@@ -352,10 +366,22 @@ int decode_f32_launch(const void* q, const void* kc, const void* vc, void* out, 
       batch > 65535 || Hq > 65535)
     return B200_ERR_UNSUPPORTED;
   DecodeF32Args a{static_cast<const float*>(q), static_cast<const float*>(kc), static_cast<const float*>(vc),
-                  static_cast<float*>(out), bt, bt_stride, lens, Hq, Hkv, bs, num_blocks, scale_log2, sink, status};
+                  static_cast<float*>(out), bt, bt_stride, lens, Hq, Hkv, bs, num_blocks, scale_log2, sink, status, 0, 0, 0};
   if (D == 32) return launch_dim<32>(a, batch, s);
   if (D == 64) return launch_dim<64>(a, batch, s);
   return launch_dim<128>(a, batch, s);
+}
+
+int window_decode_f32_launch(const WindowArgs& w, cudaStream_t s) {
+  if (w.D != w.Dv || (w.D != 32 && w.D != 64 && w.D != 128) || !aligned16(w.q) || !aligned16(w.kc) || !aligned16(w.vc) ||
+      !aligned16(w.out) || w.num_seqs > 65535 || w.Hq > 65535)
+    return B200_ERR_UNSUPPORTED;
+  DecodeF32Args a{static_cast<const float*>(w.q), static_cast<const float*>(w.kc), static_cast<const float*>(w.vc),
+                  static_cast<float*>(w.out), w.bt, w.bt_stride, w.lens, w.Hq, w.Hkv, w.bs, w.num_blocks, w.scale_log2, nullptr, w.status,
+                  w.window, w.first, w.bt_width};
+  if (w.D == 32) return launch_dim<32, true>(a, w.num_seqs, s);
+  if (w.D == 64) return launch_dim<64, true>(a, w.num_seqs, s);
+  return launch_dim<128, true>(a, w.num_seqs, s);
 }
 
 }  // namespace b200

@@ -11,7 +11,11 @@
 // key for itself: 6,620 us), half of the fp32 pipe's rate.  Scores as one chain of 64 products took 315 us, but their error
 // against 64 bits was 3.1e-7 (the general kernel's: 3.0e-7; with chains of 32: 2.6e-7).  Row tiles of 128 (RM = 8) were no
 // faster; in the general grid's order, one sequence after the other, the kernel took 80 us more.
+//
+// WINDOW (paged keys): a query sees the last `window` tokens and the first ones (window_attention.cu).  The walk goes over the tiles with
+// first tokens and then those from the start of the first row's window on; keys that no row sees are not read.
 #include "sequences.cuh"
+#include "window_attention.cuh"
 
 namespace b200 {
 namespace {
@@ -32,6 +36,8 @@ struct PrefillF32Args {
   int64_t num_blocks;
   const float* sink;         // [Hq] or null
   int32_t* status;
+  int window, first;         // WINDOW kernels
+  int bt_width;              // WINDOW kernels: entries of a table row
 };
 
 constexpr int kThreads = 128;      // 16 row groups x 8 key / column groups
@@ -43,7 +49,7 @@ __host__ __device__ constexpr size_t smem_bytes(int D, int RM) {
   return sizeof(float) * (static_cast<size_t>(bm) * (D + 4) + bn * (D + 4) + bn * D + bm * (bn + 8)) + bn * sizeof(int);
 }
 
-template <int D, int RM>
+template <int D, int RM, bool WINDOW>
 __global__ void __launch_bounds__(kThreads, RM == 2 ? 4 : D == 128 ? 2 : 3) prefill_f32_kernel(const PrefillF32Args a) {
   constexpr int BM = RM * 16, BN = tile_keys(D), CN = BN / 8, OC = D / 8;
   constexpr int QS = D + 4, PS = BN + 8;       // row strides that spread the rows of a warp over the banks
@@ -68,8 +74,13 @@ __global__ void __launch_bounds__(kThreads, RM == 2 ? 4 : D == 128 ? 2 : 3) pref
   // keys that some row of the tile sees, and that all of them see
   const int most = min(before + static_cast<int>((row0 + live - 1) / G) + 1, k_len);
   const int least = before + static_cast<int>(row0 / G) + 1;
-  const int table_keys = a.bt ? static_cast<int>(min(a.bt_stride * a.bs, static_cast<int64_t>(k_len))) : k_len;
+  const int table_keys = a.bt ? static_cast<int>(min((WINDOW ? a.bt_width : a.bt_stride) * a.bs, static_cast<int64_t>(k_len))) : k_len;
   if (a.bt && table_keys < most && tid == 0) report(a.status, B200_ERR_BOUNDS);
+  // WINDOW: first key of the first row's window, of the last row's
+  const int low = WINDOW ? max(least - a.window, 0) : 0, low_last = WINDOW ? max(before + static_cast<int>((row0 + live - 1) / G) + 1 - a.window, 0) : 0;
+  // the tile behind the one at j0
+  auto next = [&](int j0) -> int { return WINDOW && j0 + BN >= a.first && j0 + BN < low ? low / BN * BN : j0 + BN; };
+  auto seen = [&](int j, int keys) -> bool { return j < keys && (!WINDOW || j >= keys - a.window || j < a.first); };   // by a row that sees `keys`
 
   for (int i = tid; i < BM * (D / 4); i += kThreads) {
     const int r = i / (D / 4), c = i % (D / 4);
@@ -84,7 +95,7 @@ __global__ void __launch_bounds__(kThreads, RM == 2 ? 4 : D == 128 ? 2 : 3) pref
     for (int i = tid; i < BN * (D / 4); i += kThreads) {
       const int r = i / (D / 4), c = i % (D / 4), j = j0 + r;
       int64_t off = 0;
-      bool ok = j < most;
+      bool ok = j < most && (!WINDOW || j >= low || j < a.first);
       if (a.bt == nullptr) {
         off = (k0 + static_cast<int64_t>(j)) * stride + static_cast<int64_t>(kvh) * D;
       } else {
@@ -115,8 +126,9 @@ __global__ void __launch_bounds__(kThreads, RM == 2 ? 4 : D == 128 ? 2 : 3) pref
     for (int c = 0; c < OC / 2; ++c) o[i][c] = 0;
   }
 
-  load(a.k, a.k_stride, sk, QS, 0, true);
-  for (int j0 = 0; j0 < most; j0 += BN) {
+  const int begin = WINDOW && a.first == 0 ? low / BN * BN : 0;
+  load(a.k, a.k_stride, sk, QS, begin, true);
+  for (int j0 = begin; j0 < most; j0 = next(j0)) {
     load(a.v, a.v_stride, sv, D, j0, false);
     cp_async_wait<1>();
     __syncthreads();
@@ -157,13 +169,13 @@ __global__ void __launch_bounds__(kThreads, RM == 2 ? 4 : D == 128 ? 2 : 3) pref
 #pragma unroll
         for (int j = 0; j < CN; ++j) x[i][j] *= a.scale_log2;
     }
-    const bool border = j0 + BN > least;
+    const bool border = j0 + BN > least || (WINDOW && j0 < low_last && j0 + BN > a.first);
     if (border) {
 #pragma unroll
       for (int i = 0; i < RM; ++i)
 #pragma unroll
         for (int j = 0; j < CN; ++j)
-          if (j0 + tx + 8 * j >= nkeys[i]) x[i][j] = -INFINITY;
+          if (!seen(j0 + tx + 8 * j, nkeys[i])) x[i][j] = -INFINITY;
     }
     if (a.bt) {
 #pragma unroll
@@ -198,7 +210,7 @@ __global__ void __launch_bounds__(kThreads, RM == 2 ? 4 : D == 128 ? 2 : 3) pref
     }
     cp_async_wait<0>();
     __syncthreads();
-    if (j0 + BN < most) load(a.k, a.k_stride, sk, QS, j0 + BN, true);
+    if (next(j0) < most) load(a.k, a.k_stride, sk, QS, next(j0), true);
     // A weight of 0 must not meet an infinity or NaN of a value that its row does not see: tiles that some row sees only a
     // part of are searched for one, and then take the products row by row.
     bool careful = false;
@@ -236,7 +248,7 @@ __global__ void __launch_bounds__(kThreads, RM == 2 ? 4 : D == 128 ? 2 : 3) pref
       for (int j = 0; j < BN; ++j)
 #pragma unroll
         for (int i = 0; i < RM; ++i)
-          if (j0 + j < nkeys[i]) {
+          if (seen(j0 + j, nkeys[i])) {
             const float w = sp[(ty + 16 * i) * PS + j];
             const f32x2 w2 = pack2(w, w);
 #pragma unroll
@@ -270,13 +282,13 @@ __global__ void __launch_bounds__(kThreads, RM == 2 ? 4 : D == 128 ? 2 : 3) pref
   }
 }
 
-template <int D, int RM>
+template <int D, int RM, bool WINDOW>
 int launch_tiles(const PrefillF32Args& a, int max_seqlen_q, cudaStream_t s) {
   static bool configured[64] = {false};       // racing threads set the same attribute
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev >= 0 && dev < 64 && !configured[dev]) {
-    if (cudaFuncSetAttribute(prefill_f32_kernel<D, RM>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    if (cudaFuncSetAttribute(prefill_f32_kernel<D, RM, WINDOW>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                              static_cast<int>(smem_bytes(D, RM))) != cudaSuccess)
       return B200_ERR_LAUNCH;
     configured[dev] = true;
@@ -284,11 +296,11 @@ int launch_tiles(const PrefillF32Args& a, int max_seqlen_q, cudaStream_t s) {
   const int64_t tiles = (static_cast<int64_t>(max_seqlen_q) * (a.Hq / a.Hkv) + RM * 16 - 1) / (RM * 16);
   const int64_t ctas = tiles * a.Hkv * a.num_seqs;
   if (ctas > 2147483647LL) return B200_ERR_UNSUPPORTED;
-  prefill_f32_kernel<D, RM><<<static_cast<unsigned>(ctas), kThreads, smem_bytes(D, RM), s>>>(a);
+  prefill_f32_kernel<D, RM, WINDOW><<<static_cast<unsigned>(ctas), kThreads, smem_bytes(D, RM), s>>>(a);
   return launch_result();
 }
 
-template <int D>
+template <int D, bool WINDOW = false>
 int launch_rows(const PrefillF32Args& a, int max_seqlen_q, int64_t total_q, cudaStream_t s) {
   int sms = sm_count_cached();
   if (sms <= 0) sms = 148;
@@ -296,8 +308,8 @@ int launch_rows(const PrefillF32Args& a, int max_seqlen_q, int64_t total_q, cuda
   // still give every SM two (4 prompts of 100 tokens at 16/4 x 64: 18.6 us in tiles of 64, 16.5 us in tiles of 32; 8 prompts
   // of 500 tokens at 16/4 x 32: 79 and 99 us).  Sequences of up to 32 rows fill no more than the smaller tile (256 x 8 tokens behind 64 at
   // 16/16 x 128: 532 us in tiles of 64, 304 in tiles of 32).
-  if (static_cast<int64_t>(max_seqlen_q) * (a.Hq / a.Hkv) > 32 && total_q * a.Hq / 64 >= 2 * sms) return launch_tiles<D, 4>(a, max_seqlen_q, s);
-  return launch_tiles<D, 2>(a, max_seqlen_q, s);
+  if (static_cast<int64_t>(max_seqlen_q) * (a.Hq / a.Hkv) > 32 && total_q * a.Hq / 64 >= 2 * sms) return launch_tiles<D, 4, WINDOW>(a, max_seqlen_q, s);
+  return launch_tiles<D, 2, WINDOW>(a, max_seqlen_q, s);
 }
 
 // Whether the general kernel, a warp per row that reads every key, is the faster one: short portions leave most of a 32-row tile
@@ -333,11 +345,23 @@ int prefill_f32_launch(const void* q, const void* k, const void* v, void* out, i
     return B200_ERR_UNSUPPORTED;
   PrefillF32Args a{static_cast<const float*>(q), static_cast<const float*>(kp), static_cast<const float*>(vp),
                    static_cast<float*>(out), q_stride, k_stride, v_stride, cu_q, cu_k, num_seqs, Hq, Hkv,
-                   scale * 1.4426950408889634f, bt, bt_stride, bs, num_blocks, sink, status};
+                   scale * 1.4426950408889634f, bt, bt_stride, bs, num_blocks, sink, status, 0, 0, 0};
   if (general_is_faster(a, Dqk, total_q, max_seqlen_q, max_seqlen_k)) return B200_ERR_UNSUPPORTED;
   if (Dqk == 32) return launch_rows<32>(a, max_seqlen_q, total_q, s);
   if (Dqk == 64) return launch_rows<64>(a, max_seqlen_q, total_q, s);
   return launch_rows<128>(a, max_seqlen_q, total_q, s);
+}
+
+int window_prefill_f32_launch(const WindowArgs& w, int64_t total_q, int max_seqlen_q, cudaStream_t s) {
+  if (w.D != w.Dv || (w.D != 32 && w.D != 64 && w.D != 128) || static_cast<int64_t>(w.num_seqs) * w.Hkv > 2147483647LL || !aligned16(w.q) ||
+      !aligned16(w.kc) || !aligned16(w.vc) || !aligned16(w.out) || w.q_stride % 4)
+    return B200_ERR_UNSUPPORTED;
+  PrefillF32Args a{static_cast<const float*>(w.q), static_cast<const float*>(w.kc), static_cast<const float*>(w.vc), static_cast<float*>(w.out),
+                   w.q_stride, 0, 0, w.cu_q, w.cu_k, w.num_seqs, w.Hq, w.Hkv, w.scale_log2, w.bt, w.bt_stride, w.bs, w.num_blocks, nullptr, w.status,
+                   w.window, w.first, w.bt_width};
+  if (w.D == 32) return launch_rows<32, true>(a, max_seqlen_q, total_q, s);
+  if (w.D == 64) return launch_rows<64, true>(a, max_seqlen_q, total_q, s);
+  return launch_rows<128, true>(a, max_seqlen_q, total_q, s);
 }
 
 }  // namespace b200

@@ -108,6 +108,18 @@ int general(const WindowArgs& a, int max_seqlen_q, int32_t dtype, cudaStream_t s
   return dtype == B200_DTYPE_F32 ? launch_general<float>(a, max_seqlen_q, s) : launch_general<__nv_bfloat16>(a, max_seqlen_q, s);
 }
 
+int dispatch(const WindowArgs& given_args, int64_t total_q, int max_seqlen_q, int32_t dtype, cudaStream_t s) {
+  WindowArgs a = given_args;
+  int rc = B200_ERR_UNSUPPORTED;
+  if (static_cast<int64_t>(a.bt_width) * a.bs <= kMaxPosition) {
+    if (a.window > kMaxPosition) a.window = kMaxPosition;
+    if (a.first > kMaxPosition) a.first = kMaxPosition;
+    if (dtype == B200_DTYPE_BF16) rc = a.cu_q != nullptr ? window_prefill_launch(a, total_q, s) : window_decode_launch(a, s);
+    else rc = a.cu_q != nullptr ? window_prefill_f32_launch(a, total_q, max_seqlen_q, s) : window_decode_f32_launch(a, s);
+  }
+  return rc == B200_ERR_UNSUPPORTED ? general(given_args, max_seqlen_q, dtype, s) : rc;
+}
+
 }  // namespace
 }  // namespace b200
 
@@ -132,7 +144,7 @@ extern "C" int b200_window_attention(const void* q, int64_t q_token_stride, cons
   if (total_q < 0 || max_seqlen_q < 0) return B200_ERR_ARG;
   if (num_seqs == 0 || total_q == 0 || max_seqlen_q == 0) return B200_OK;
   if (!cu_seqlens_q || !given(a)) return B200_ERR_ARG;
-  return general(a, max_seqlen_q, dtype, static_cast<cudaStream_t>(stream));
+  return dispatch(a, total_q, max_seqlen_q, dtype, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int b200_window_decode(const void* q, const void* k_cache, const void* v_cache, void* out, const int32_t* block_tables,
@@ -154,5 +166,5 @@ extern "C" int b200_window_decode(const void* q, const void* k_cache, const void
   if (rc != B200_OK) return rc;
   if (batch == 0) return B200_OK;
   if (!given(a)) return B200_ERR_ARG;
-  return general(a, 1, dtype, static_cast<cudaStream_t>(stream));
+  return dispatch(a, batch, 1, dtype, static_cast<cudaStream_t>(stream));
 }

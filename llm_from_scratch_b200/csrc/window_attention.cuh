@@ -23,4 +23,13 @@ struct WindowArgs {
   int32_t* status;
 };
 
+// The tiled kernels count positions in 32 bits: a window or a number of first tokens beyond every position is cut to this one.
+constexpr int kMaxPosition = 1 << 30;
+
+// Launches of the tiled kernels; B200_ERR_UNSUPPORTED: a shape, page size or alignment that the general kernel takes.
+int window_prefill_launch(const WindowArgs& a, int64_t total_q, cudaStream_t s);                       // bf16, head sizes 64 and 128
+int window_decode_launch(const WindowArgs& a, cudaStream_t s);                                         // bf16, head sizes 64 and 128
+int window_prefill_f32_launch(const WindowArgs& a, int64_t total_q, int max_seqlen_q, cudaStream_t s); // head sizes 32, 64 and 128
+int window_decode_f32_launch(const WindowArgs& a, cudaStream_t s);                                     // head sizes 32, 64 and 128
+
 }  // namespace b200
