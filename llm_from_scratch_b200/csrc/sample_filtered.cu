@@ -8,16 +8,18 @@
 // Rows with T <= 0 and rows without any weight (no logit above -inf) take the first of the highest logits.  NaN counts as -inf.
 //
 // Weights are computed in 64 bits and held as whole numbers of 2^-S, S as large as their sum allows (45 bits at 131,072
-// tokens): sums of whole numbers do not depend on their order, so the borders fall at the same token whatever the launch looks like.
+// tokens, no more in the clustered kernel): sums of whole numbers do not depend on their order, so the borders fall at the same token whatever the launch looks like.
 //
 // A cluster of CTAs shares a row, whose logits stay in shared memory: a thread owns a run of neighbouring tokens.  Borders by value (top-k with
-// ones as masses, top-p with the weights) are found with a histogram over the distance from the maximum, in steps of T / 64, and, if the
+// ones as masses, top-p with the weights) are found with a histogram over the distance from the maximum, in steps of T / 128, and, if the
 // border's bin holds more than a few tokens, over ever finer ranges of the logits' bits; what is left is sorted.  The border of the draw is
 // found by sums over the threads' runs.  Histograms hold a weight in three parts of 16 bits or more, each a 32-bit counter: shared memory adds
 // 32 bits at a time.
 //
 // Bound by the reads for large rows in principle; in fact by the weights (ten 64-bit operations each) and the histogram's additions.
 #include <cooperative_groups.h>
+
+#include <type_traits>
 
 #include "common.cuh"
 
@@ -52,19 +54,36 @@ __device__ __forceinline__ float key_value(uint32_t k) { return __uint_as_float(
 // rows that fit the shared memory of a cluster
 // ---------------------------------------------------------------------------------------------
 constexpr int kRowThreads = 512, kRowWarps = kRowThreads / 32;
-constexpr int kBins = 2048;
-constexpr int kList = 512;           // tokens that are sorted at most
-constexpr double kMagic = 6755399441055744.0;      // 1.5 * 2^52: added, it leaves the nearest whole number in the low bits
+constexpr int kBins = 4096, kOwnBins = kBins / kRowThreads;        // of the histogram of counts, two to a word
+constexpr int kSteps = 2048, kOwnSteps = kSteps / kRowThreads;     // of the histograms of weights
+constexpr int kList = 1024, kOwnList = kList / kRowThreads;        // tokens that are sorted at most
+constexpr float kPerUnit = 128.f;                                   // bins per distance T from the maximum: 32 T and the last bin
+constexpr double kMagic = 6755399441055744.0;                       // 1.5 * 2^52: added, it leaves the nearest whole number in the low bits
 
-struct RowShared {
+struct alignas(16) RowShared {      // the logits lie behind it in 16-byte pieces
   double table[64];                  // 2^(i / 64)
-  uint32_t hist[3][kBins];
-  unsigned long long list_key[kList], list_mass[kList];
-  unsigned long long parts[8];       // of the CTAs of the cluster
-  unsigned long long scan[kRowWarps];
+  union {
+    uint32_t hist[kSteps];           // counts: bins 2 i and 2 i + 1; weights: their bits 0 .. 15
+    unsigned long long sorted_key[kList];
+  };
+  union {                            // never in use together
+    uint32_t upper[2][kSteps];       // weights: their bits 16 .. 31 and from 32 on
+    struct {
+      unsigned long long key[kList], mass[kList];
+    } list;
+  };
+  unsigned long long sorted_mass[kList];
+  unsigned long long drawn[kRowThreads];   // kept weights of the list, by the thread that owns the token
+  unsigned long long parts[2][8][3]; // of the CTAs of the cluster, in turns
+  unsigned long long scan[kRowWarps][3];
   unsigned long long found_key, found_left;
   uint32_t list_size, lo_key, hi_key;
+  uint32_t bin_lo, before_lo, bin_hi, upto_hi;       // the bracket, the tokens in front of it and up to its end
+  int bin_k, left_k, count_k, step_at;
+  float mass_k, spread_k;
 };
+
+static_assert(sizeof(RowShared) % 16 == 0, "the logits behind it are read in 16-byte pieces");
 
 // Shape of a row in the cluster: tokens of a CTA, of a thread, and the stride of the threads' runs (an odd number of 16-byte pieces, so that
 // the lanes of a warp read different banks).
@@ -80,355 +99,808 @@ __host__ __device__ inline RowShape row_shape(int vocab, int ranks) {
 }
 inline size_t row_smem(int vocab, int ranks) { return sizeof(RowShared) + static_cast<size_t>(kRowThreads) * row_shape(vocab, ranks).stride * 4; }
 
+__device__ __forceinline__ int min_of(int x, int y) { return x < y ? x : y; }
+__device__ __forceinline__ int max_of(int x, int y) { return x > y ? x : y; }
+
+// 2^(i / 64)
+__device__ const double kTable[64] = {
+    1.0, 1.0108892860517005, 1.0218971486541166, 1.0330248790212284,
+    1.0442737824274138, 1.0556451783605572, 1.0671404006768237, 1.0787607977571199,
+    1.0905077326652577, 1.102382583307841, 1.1143867425958924, 1.1265216186082418,
+    1.1387886347566916, 1.1511892299529827, 1.1637248587775775, 1.1763969916502812,
+    1.189207115002721, 1.202156731452703, 1.215247359980469, 1.22848053610687,
+    1.241857812073484, 1.255380757024691, 1.2690509571917332, 1.2828700160787783,
+    1.2968395546510096, 1.3109612115247644, 1.3252366431597413, 1.339667524053303,
+    1.3542555469368927, 1.3690024229745905, 1.383909881963832, 1.3989796725383112,
+    1.4142135623730951, 1.42961333839197, 1.4451808069770467, 1.460917794180647,
+    1.4768261459394993, 1.4929077282912648, 1.5091644275934228, 1.5255981507445384,
+    1.5422108254079407, 1.559004400237837, 1.5759808451078865, 1.593142151342267,
+    1.6104903319492543, 1.6280274218573478, 1.645755478153965, 1.6636765803267364,
+    1.681792830507429, 1.7001063537185235, 1.718619298122478, 1.7373338352737062,
+    1.7562521603732995, 1.7753764925265212, 1.7947090750031072, 1.8142521755003989,
+    1.8340080864093424, 1.8539791250833855, 1.8741676341103, 1.8945759815869656,
+    1.9152065613971474, 1.9360617934922943, 1.9571441241754002, 1.978456026387951};
+
+// The weight in units of 2^-S: 2^(n / 64) 2^(r / 64) with |r| <= 1/2, the second factor by its series up to r^4 (error 4e-14).
+__device__ __forceinline__ double weight_of(float x, float top, double max, double factor, float reach, int S, const double* table) {
+  const double y = (static_cast<double>(x) - max) * factor;
+  const double t = y + kMagic, r = y - (t - kMagic);
+  const int n = __double2loint(t);
+  constexpr double b = 0.010830424696249145;             // ln 2 / 64
+  const double q = fma(r, fma(r, fma(r, fma(r, b * b * b * b / 24, b * b * b / 6), b * b / 2), b), 1.0);
+  const double v = table[n & 63] * q;
+  return top - x > reach ? 0.0 : __hiloint2double(__double2hiint(v) + (((n >> 6) + S) << 20), __double2loint(v));
+}
+
+// What the kernel's parts know of a row.
+struct Row {
+  RowShared* sh;
+  float* own;                        // the thread's logits
+  RowShape shape;
+  int rank, ranks, begin, mine;      // place in the cluster, first token of the CTA and of the thread
+  int S, turn;                       // turn of `parts`: two uses in a row do not meet, and a third comes behind a barrier
+  float top, temperature, step, reach;
+  double max, factor, floor_w;
+  float edge;                        // kept: tokens above the border, and of those at it the ones up to a token
+  int edge_token;
+
+  __device__ __forceinline__ RowShared* other(int r) const { return cooperative_groups::this_cluster().map_shared_rank(sh, r); }
+  __device__ __forceinline__ void sync() const {
+    if (ranks > 1) cooperative_groups::this_cluster().sync();
+    else __syncthreads();
+  }
+  __device__ __forceinline__ bool kept(float x, int i) const { return x > edge || (x == edge && i <= edge_token); }
+  __device__ __forceinline__ double weight(float x) const { return weight_of(x, top, max, factor, reach, S, sh->table); }
+  // below 2^51; 0 for weights below e^-32
+  static __device__ __forceinline__ unsigned long long rounded(double w) {
+    return static_cast<unsigned long long>(__double_as_longlong(w + 4503599627370496.0)) & 0xfffffffffffffull;
+  }
+  // Bin 0: the maximum; bin b: distances above (b - 1) / 128 and up to b / 128 times T; the last one: all beyond, whose weights round to 0.
+  __device__ __forceinline__ int bin_of(float x) const {               // never falls as x falls
+    return min_of(__float2int_ru((top - x) * step), kBins - 1);      // saturates
+  }
+  static __device__ __forceinline__ unsigned long long composite(float x, int i) {
+    return static_cast<unsigned long long>(order_key(x)) << 32 | static_cast<uint32_t>(~i);
+  }
+  __device__ __forceinline__ void set_edge(unsigned long long c) {
+    edge = key_value(static_cast<uint32_t>(c >> 32));
+    edge_token = static_cast<int>(~static_cast<uint32_t>(c));
+  }
+  template <typename F>
+  __device__ __forceinline__ void each(F f) const {      // f(four logits, the first one's token) over the thread's run
+#pragma unroll 1
+    for (int i = 0; i < shape.run; i += 4) {
+      const float4 t = *reinterpret_cast<const float4*>(own + i);
+      const float v[4] = {t.x, t.y, t.z, t.w};
+      f(v, mine + i);
+    }
+  }
+};
+
+// Sum over the warp, in all lanes: three parts of 24 bits, whose sums fit 32.
+__device__ __forceinline__ unsigned long long warp_total(unsigned long long v) {
+  const uint32_t lo = __reduce_add_sync(0xffffffffu, static_cast<uint32_t>(v) & 0xffffffu);
+  const uint32_t mid = __reduce_add_sync(0xffffffffu, static_cast<uint32_t>(v >> 24) & 0xffffffu);
+  const uint32_t hi = __reduce_add_sync(0xffffffffu, static_cast<uint32_t>(v >> 48));
+  return lo + (static_cast<unsigned long long>(mid) << 24) + (static_cast<unsigned long long>(hi) << 48);
+}
+template <typename U>
+__device__ __forceinline__ U warp_upto(U v) {            // inclusive running sum over the lanes
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const U y = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += y;
+  }
+  return v;
+}
+
+// A row's kernel runs through most of its code once, so fetching instructions sets the pace of small rows: of the stalls of one row of 32,000 more
+// than half are for instructions.  Calls out of line do not help, as they put the row's values into memory (256 rows of 131,072: 435 us
+// against 341).
+
+// Running sum over the CTA's threads, inclusive, and the CTA's sum.
+struct RunUp {
+  unsigned long long upto, all;
+};
+__device__ __noinline__ RunUp run_up(RowShared& sh, unsigned long long v) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  v = warp_upto(v);
+  __syncthreads();
+  if (lane == 31) sh.scan[warp][0] = v;
+  __syncthreads();
+  const unsigned long long upto = warp_upto(lane < kRowWarps ? sh.scan[lane][0] : 0ull);
+  const unsigned long long before = __shfl_sync(0xffffffffu, upto, warp > 0 ? warp - 1 : 0);
+  return {warp > 0 ? v + before : v, __shfl_sync(0xffffffffu, upto, kRowWarps - 1)};
+}
+
+// Sorts the list into sorted_key / sorted_mass: a token's place is the number of those before it.
+__device__ __forceinline__ void sort_list(RowShared& sh, int size) {
+#pragma unroll 1
+  for (int i = threadIdx.x; i < size; i += kRowThreads) {
+    const unsigned long long key = sh.list.key[i];
+    int place = 0;
+#pragma unroll 4
+    for (int j = 0; j < size; ++j) place += sh.list.key[j] > key;
+    sh.sorted_key[place] = key;
+    sh.sorted_mass[place] = sh.list.mass[i];
+  }
+  __syncthreads();
+}
+
+// What the tokens of a group of four add to a running mass: ones for kept tokens equal to `x0`; or kept weights above the floor; or ones for kept
+// tokens of any weight above the floor.
+enum Mass { kTies, kWeights, kAny };
+__device__ __forceinline__ void mass_of_four(const Row& w, Mass kind, float x0, const float (&v)[4], int i, unsigned long long (&m)[4]) {
+  bool in[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) in[j] = w.kept(v[j], i + j), m[j] = 0;
+  if (!(in[0] || in[1] || in[2] || in[3])) return;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const double g = w.weight(v[j]);
+    const bool counts = in[j] && g >= w.floor_w;
+    if (kind == kTies) m[j] = in[j] && v[j] == x0;
+    else if (kind == kAny) m[j] = counts && static_cast<double>(v[j]) - w.max > -745.13 * w.temperature;
+    else m[j] = counts ? Row::rounded(g) : 0ull;
+  }
+}
+
+// The first token at which the running mass reaches its target, by token: with `known` the thread's own mass is `sum`.  The target is `ties` for
+// kTies, 1 for kAny, else u times the whole.  -1 in all threads of the cluster but one.
+__device__ __forceinline__ int locate(Row& w, Mass kind, float x0, unsigned long long ties, float u, bool known, unsigned long long sum) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  RowShared& sh = *w.sh;
+  if (!known) {
+    sum = 0;
+    w.each([&](const float (&v)[4], int i) {
+      unsigned long long m[4];
+      mass_of_four(w, kind, x0, v, i, m);
+      sum += m[0] + m[1] + (m[2] + m[3]);
+    });
+  }
+  const RunUp run_sum = run_up(sh, sum);
+  unsigned long long upto = run_sum.upto, total = run_sum.all;
+  if (w.ranks > 1) {
+    if (threadIdx.x < w.ranks) w.other(threadIdx.x)->parts[w.turn][w.rank][0] = total;
+    w.sync();
+    const unsigned long long part = lane < w.ranks ? sh.parts[w.turn][lane][0] : 0ull;
+    upto += warp_total(lane < w.rank ? part : 0ull);
+    total = warp_total(part);
+    w.turn ^= 1;
+  }
+  unsigned long long target = kind == kTies ? ties : kind == kAny ? 1ull
+      : static_cast<unsigned long long>(static_cast<double>(u) * static_cast<double>(total)) + 1;
+  if (target > total) target = total;
+  const unsigned owner = __ballot_sync(0xffffffffu, upto >= target && upto - sum < target);
+  if (owner == 0) return -1;
+  // the owner's run, a group of four per lane
+  const int src = __ffs(owner) - 1;
+  unsigned long long left = __shfl_sync(0xffffffffu, target - (upto - sum), src);
+  const float* run = w.own + (src - lane) * w.shape.stride;
+  const int first = w.mine + (src - lane) * w.shape.run;
+#pragma unroll 1
+  for (int base = 0; base < w.shape.run; base += 128) {
+    const int i = base + lane * 4;
+    unsigned long long m[4] = {0, 0, 0, 0};
+    if (i < w.shape.run) {
+      const float4 t = *reinterpret_cast<const float4*>(run + i);
+      const float v[4] = {t.x, t.y, t.z, t.w};
+      mass_of_four(w, kind, x0, v, first + i, m);
+    }
+    const unsigned long long four = m[0] + m[1] + (m[2] + m[3]), up = warp_upto(four);
+    const bool here = up >= left && up - four < left;
+    if (__any_sync(0xffffffffu, here)) {
+      int j = 0;
+      unsigned long long rest = left - (up - four);
+#pragma unroll
+      for (int c = 0; c < 3; ++c)
+        if (j == c && rest > m[c]) rest -= m[c], ++j;
+      return here ? first + i + j : -1;
+    }
+    left -= __shfl_sync(0xffffffffu, up, 31);
+  }
+  return -1;
+}
+
+// The border by value in any row: the edge becomes the first kept token of the bins from .. to, from the front of the order, at which the running
+// mass (ones with `ones`, else the weights) reaches `target`.  Histograms of the masses over fine steps of these bins, then over ever finer
+// ranges of the logits' bits, until the border's place fits the list.
+__device__ __forceinline__ void cut(Row& w, const bool ones, unsigned long long target, const int from_bin, const int to_bin) {
+  const int tid = threadIdx.x, lane = tid & 31;
+  RowShared& sh = *w.sh;
+  int level = 0, shift = 0;
+  uint32_t lo_key = 0, hi_key = 0xffffffffu;
+  const float origin = from_bin - 1.f, scale = static_cast<float>(kSteps - 1) / (to_bin - from_bin + 1);
+  auto place = [&](float x, int i) -> int {              // at this level; -1: not a candidate
+    int s;
+    if (level == 0) {
+      const int b = w.bin_of(x);
+      s = b < from_bin || b > to_bin ? -1 : max_of(0, min_of(kSteps - 1, __float2int_ru(((w.top - x) * w.step - origin) * scale)));
+    } else {
+      const uint32_t key = order_key(x);
+      s = key < lo_key || key > hi_key ? -1 : static_cast<int>((hi_key - key) >> shift);
+    }
+    return s >= 0 && w.kept(x, i) ? s : -1;
+  };
+  auto mass_of = [&](float x) -> unsigned long long { return ones ? 1ull : Row::rounded(w.weight(x)); };
+  for (;;) {
+    w.sync();                                            // the list of an earlier use has been read
+    for (int i = tid; i < kSteps; i += kRowThreads) sh.hist[i] = sh.upper[0][i] = sh.upper[1][i] = 0;
+    __syncthreads();
+#pragma unroll 1
+    for (int i = 0; i < w.shape.run; ++i) {
+      const float x = w.own[i];
+      const int s = place(x, w.mine + i);
+      if (s < 0) continue;
+      const unsigned long long m = mass_of(x);
+      const uint32_t m0 = m & 0xffff, m1 = (m >> 16) & 0xffff, m2 = static_cast<uint32_t>(m >> 32);
+      if (m0) atomicAdd(&sh.hist[s], m0);
+      if (m1) atomicAdd(&sh.upper[0][s], m1);
+      if (m2) atomicAdd(&sh.upper[1][s], m2);
+    }
+    w.sync();
+    unsigned long long h[kOwnSteps], sum = 0;
+#pragma unroll
+    for (int j = 0; j < kOwnSteps; ++j) {
+      h[j] = 0;
+#pragma unroll 1
+      for (int r = 0; r < w.ranks; ++r) {
+        const RowShared* from = w.other(r);
+        const int at = tid * kOwnSteps + j;
+        h[j] += from->hist[at] + (static_cast<unsigned long long>(from->upper[0][at]) << 16) + (static_cast<unsigned long long>(from->upper[1][at]) << 32);
+      }
+      sum += h[j];
+    }
+    const unsigned long long upto = run_up(sh, sum).upto;
+    if (upto >= target && upto - sum < target) {         // one thread of every CTA
+      unsigned long long left = target - (upto - sum);
+      int s = tid * kOwnSteps;
+#pragma unroll
+      for (int j = 0; j < kOwnSteps - 1; ++j) {
+        if (left <= h[j]) break;
+        left -= h[j];
+        ++s;
+      }
+      sh.step_at = s;
+      sh.found_left = left;
+      sh.list_size = 0;
+      sh.lo_key = 0xffffffffu;
+      sh.hi_key = 0;
+    }
+    w.sync();                                            // the histograms have been read, and the list is empty
+    const int step_at = sh.step_at;
+    target = sh.found_left;
+    RowShared* lead = w.other(0);
+    uint32_t least = 0xffffffffu, most = 0;
+#pragma unroll 1
+    for (int i = 0; i < w.shape.run; ++i) {
+      const float x = w.own[i];
+      if (place(x, w.mine + i) != step_at) continue;
+      const unsigned long long m = mass_of(x);
+      if (m == 0) continue;
+      const uint32_t key = order_key(x), at = atomicAdd(&lead->list_size, 1u);
+      least = min(least, key);
+      most = key > most ? key : most;
+      if (at < kList) lead->list.key[at] = Row::composite(x, w.mine + i), lead->list.mass[at] = m;
+    }
+    least = __reduce_min_sync(0xffffffffu, least);
+    most = __reduce_max_sync(0xffffffffu, most);
+    if (lane == 0 && most != 0) atomicMin(&lead->lo_key, least), atomicMax(&lead->hi_key, most);
+    w.sync();
+    const int size = static_cast<int>(lead->list_size);
+    const uint32_t least_all = lead->lo_key, most_all = lead->hi_key;
+    if (size <= kList) {
+      if (w.rank == 0) {
+        sort_list(sh, size);
+        unsigned long long m[kOwnList], own_sum = 0;
+#pragma unroll
+        for (int j = 0; j < kOwnList; ++j) {
+          const int i = tid * kOwnList + j;
+          m[j] = i < size ? sh.sorted_mass[i] : 0;
+          own_sum += m[j];
+        }
+        unsigned long long up = run_up(sh, own_sum).upto - own_sum;
+#pragma unroll
+        for (int j = 0; j < kOwnList; ++j) {
+          if (up < target && up + m[j] >= target)
+            for (int r = 0; r < w.ranks; ++r) w.other(r)->found_key = sh.sorted_key[tid * kOwnList + j];
+          up += m[j];
+        }
+      }
+      w.sync();
+      w.set_edge(sh.found_key);
+      return;
+    }
+    if (least_all == most_all) {                         // equal logits: so many of them, by token
+      const float x0 = key_value(least_all);
+      const unsigned long long one = mass_of(x0);
+      const int token = locate(w, kTies, x0, (target + one - 1) / one, 0.f, false, 0);
+      if (token >= 0)
+        for (int r = 0; r < w.ranks; ++r) w.other(r)->found_key = static_cast<uint32_t>(~token);
+      w.sync();
+      w.edge = x0;
+      w.edge_token = static_cast<int>(~static_cast<uint32_t>(sh.found_key));
+      return;
+    }
+    lo_key = least_all, hi_key = most_all;               // logits of one place: a range of bits
+    const int width = 32 - __clz(hi_key - lo_key);
+    shift = width > 11 ? width - 11 : 0;
+    ++level;
+  }
+}
+
+// Three sums over the cluster, the same in all threads.
+struct Sums {
+  unsigned long long v[3];
+};
+__device__ __forceinline__ Sums combine(Row& w, Sums s) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  RowShared& sh = *w.sh;
+#pragma unroll 1
+  for (int stage = 0; stage < 3; ++stage) {
+#pragma unroll
+    for (int c = 0; c < 3; ++c) s.v[c] = warp_total(s.v[c]);
+    if (stage == 0) {
+      __syncthreads();
+      if (lane == 0)
+#pragma unroll
+        for (int c = 0; c < 3; ++c) sh.scan[warp][c] = s.v[c];
+      __syncthreads();
+#pragma unroll
+      for (int c = 0; c < 3; ++c) s.v[c] = lane < kRowWarps ? sh.scan[lane][c] : 0ull;
+    } else if (stage == 1) {
+      if (w.ranks == 1) break;
+      if (threadIdx.x < w.ranks)
+#pragma unroll
+        for (int c = 0; c < 3; ++c) w.other(threadIdx.x)->parts[w.turn][w.rank][c] = s.v[c];
+      w.sync();
+#pragma unroll
+      for (int c = 0; c < 3; ++c) s.v[c] = lane < w.ranks ? sh.parts[w.turn][lane][c] : 0ull;
+      w.turn ^= 1;
+    }
+  }
+  return s;
+}
+__device__ __forceinline__ uint32_t combine_max(Row& w, uint32_t v) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  RowShared& sh = *w.sh;
+  v = __reduce_max_sync(0xffffffffu, v);
+  __syncthreads();
+  if (lane == 0) sh.scan[warp][0] = v;
+  __syncthreads();
+  v = __reduce_max_sync(0xffffffffu, lane < kRowWarps ? static_cast<uint32_t>(sh.scan[lane][0]) : 0u);
+  if (w.ranks > 1) {
+    if (threadIdx.x < w.ranks) w.other(threadIdx.x)->parts[w.turn][w.rank][0] = v;
+    w.sync();
+    v = __reduce_max_sync(0xffffffffu, lane < w.ranks ? static_cast<uint32_t>(sh.parts[w.turn][lane][0]) : 0u);
+    w.turn ^= 1;
+  }
+  return v;
+}
+
+// Sums without a list: kept weights in front of the bins lo .. hi, behind them and in them.
+__device__ __forceinline__ Sums sum_weights(Row& w, const float y_lo, const float y_hi) {
+  Sums s = {{0, 0, 0}};
+  w.each([&](const float (&v)[4], int i) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float y = (w.top - v[j]) * w.step;
+      if (w.kept(v[j], i + j)) s.v[y <= y_lo ? 0 : y <= y_hi ? 2 : 1] += Row::rounded(w.weight(v[j]));
+    }
+  });
+  return combine(w, s);
+}
+
+// The first of the highest logits, in all threads.
+__device__ __forceinline__ int first_highest(Row& w, int vocab) {
+  uint32_t first = 0;
+  w.each([&](const float (&v)[4], int i) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (v[j] == w.top && i + j < vocab) first = first > ~static_cast<uint32_t>(i + j) ? first : ~static_cast<uint32_t>(i + j);
+  });
+  return static_cast<int>(~combine_max(w, first));
+}
+
 template <typename T>
 __global__ void __launch_bounds__(kRowThreads, 2) sample_row_kernel(const SampleArgs a) {
-  namespace cg = cooperative_groups;
   extern __shared__ __align__(16) uint8_t smem[];
   RowShared& sh = *reinterpret_cast<RowShared*>(smem);
   float* data = reinterpret_cast<float*>(smem + sizeof(RowShared));
-  cg::cluster_group cluster = cg::this_cluster();
-  const int rank = cluster.block_rank(), ranks = cluster.num_blocks();
-  const int row = blockIdx.x / ranks, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, V = a.vocab;
-  const RowShape shape = row_shape(V, ranks);
-  const int begin = rank * shape.slice;                  // first token of the CTA
-  const int mine = begin + tid * shape.run;              // of the thread
-  float* own = data + tid * shape.stride;
-  auto sync = [&]() {
-    if (ranks > 1) cluster.sync();
-    else __syncthreads();
-  };
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, V = a.vocab;
+  Row w;
+  w.sh = &sh;
+  w.rank = cooperative_groups::this_cluster().block_rank(), w.ranks = cooperative_groups::this_cluster().num_blocks();
+  const int row = blockIdx.x / w.ranks, rank = w.rank, ranks = w.ranks;
+  w.shape = row_shape(V, ranks);
+  const RowShape shape = w.shape;
+  const int begin = rank * shape.slice;
+  w.begin = begin, w.mine = begin + tid * shape.run, w.own = data + tid * shape.stride;
+  w.S = a.bits, w.turn = 0;
+  w.edge = -INFINITY, w.edge_token = 0x7fffffff;
+  w.temperature = fminf(a.temperatures[row], 1e30f);     // beyond that all finite logits weigh the same
+  const float p = a.top_p ? a.top_p[row] : 1.f, u = fminf(a.uniforms[row], 1.f);
+  int k = a.top_k ? a.top_k[row] : 0;
+  const float floor_w = a.min_p ? a.min_p[row] : 0.f;
+  w.floor_w = (floor_w > 1.f ? 1.0 : floor_w > 0.f ? static_cast<double>(floor_w) : 0.0) * static_cast<double>(1ull << a.bits);
 
   // ---- the CTA's logits; NaN and what lies behind the row as -inf
+  float top = -INFINITY;
   {
     const T* x = static_cast<const T*>(a.logits) + row * a.row_stride + begin;
     const int n = min(shape.slice, V - begin);           // may be negative
     auto clean = [](float v) { return v != v ? -INFINITY : v; };
     const int all = kRowThreads * shape.run;
-    constexpr int W = 16 / sizeof(T);
+    constexpr int W = 16 / sizeof(T), STEP = kRowThreads * W;
     const bool wide = reinterpret_cast<uintptr_t>(x) % 16 == 0;
-    for (int i = tid * W; i < all; i += kRowThreads * W) {
-      float v[W];
-      if (wide && i + W <= n) {
-        const uint4 raw = __ldg(reinterpret_cast<const uint4*>(x + i));
-        const T* e = reinterpret_cast<const T*>(&raw);
+    // owner and place of a group of four, kept up from trip to trip instead of divided out
+    int owner = (tid * W) / shape.run, at = (tid * W) % shape.run;
+    const int more = STEP / shape.run, rest = STEP % shape.run;
+    auto put = [&](const float (&v)[W]) {
 #pragma unroll
-        for (int j = 0; j < W; ++j) v[j] = clean(to_float<T>(e[j]));
-      } else {
-#pragma unroll
-        for (int j = 0; j < W; ++j) v[j] = i + j < n ? clean(to_float<T>(x[i + j])) : -INFINITY;
-      }
+      for (int j = 0; j < W; ++j) top = fmaxf(top, v[j]);
+      int o = owner, c = at;
 #pragma unroll
       for (int j = 0; j < W; j += 4) {
-        const int owner = (i + j) / shape.run, at = (i + j) % shape.run;
-        if (owner < kRowThreads) *reinterpret_cast<float4*>(data + owner * shape.stride + at) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+        if (o < kRowThreads) *reinterpret_cast<float4*>(data + o * shape.stride + c) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+        c += 4;
+        if (c == shape.run) c = 0, ++o;
+      }
+      owner += more, at += rest;
+      if (at >= shape.run) at -= shape.run, ++owner;
+    };
+    int i = tid * W;
+    if (wide) {
+      constexpr int AHEAD = 4;                           // loads in flight
+#pragma unroll 1
+      for (; i + (AHEAD - 1) * STEP + W <= n; i += AHEAD * STEP) {
+        uint4 raw[AHEAD];
+#pragma unroll
+        for (int c = 0; c < AHEAD; ++c) raw[c] = __ldg(reinterpret_cast<const uint4*>(x + i + c * STEP));
+#pragma unroll
+        for (int c = 0; c < AHEAD; ++c) {
+          const T* e = reinterpret_cast<const T*>(&raw[c]);
+          float v[W];
+#pragma unroll
+          for (int j = 0; j < W; ++j) v[j] = clean(to_float<T>(e[j]));
+          put(v);
+        }
       }
     }
-    if (tid < 64) sh.table[tid] = exp2(tid / 64.0);
+#pragma unroll 1
+    for (; i < all; i += STEP) {
+      float v[W];
+#pragma unroll
+      for (int j = 0; j < W; ++j) v[j] = i + j < n ? clean(to_float<T>(x[i + j])) : -INFINITY;
+      put(v);
+    }
+    if (tid < 64) sh.table[tid] = kTable[tid];
+    sh.drawn[tid] = 0;
+    for (int j = tid; j < kSteps; j += kRowThreads) sh.hist[j] = 0;
     if (tid == 0) sh.list_size = 0;
   }
-  __syncthreads();
-  auto each = [&](auto f) {                              // f(logit, token) over the thread's run
-    for (int i = 0; i < shape.run; i += 4) {
-      const float4 v = *reinterpret_cast<const float4*>(own + i);
-      f(v.x, mine + i), f(v.y, mine + i + 1), f(v.z, mine + i + 2), f(v.w, mine + i + 3);
-    }
-  };
-  auto composite = [](float x, int i) -> unsigned long long {
-    return static_cast<unsigned long long>(order_key(x)) << 32 | static_cast<uint32_t>(~i);
-  };
-  // over the cluster, the same in all threads; what parts held is lost
-  auto combine = [&](unsigned long long v, bool max) -> unsigned long long {
-    auto join = [&](unsigned long long x, unsigned long long y) { return max ? (x > y ? x : y) : x + y; };
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v = join(v, __shfl_xor_sync(0xffffffffu, v, o));
-    if (lane == 0) sh.scan[warp] = v;
-    __syncthreads();
-    v = sh.scan[0];
-    for (int w = 1; w < kRowWarps; ++w) v = join(v, sh.scan[w]);
-    if (ranks > 1) {
-      if (tid < ranks) *cluster.map_shared_rank(&sh.parts[rank], tid) = v;
-      cluster.sync();
-      v = sh.parts[0];
-      for (int r = 1; r < ranks; ++r) v = join(v, sh.parts[r]);
-    }
-    sync();                                              // scan and parts may be written again
-    return v;
-  };
-
-  unsigned long long best = 0;
-  each([&](float x, int i) {
-    const unsigned long long c = composite(x, i);
-    best = c > best ? c : best;
-  });
-  best = combine(best, true);
-  const float temperature = a.temperatures[row], top = key_value(static_cast<uint32_t>(best >> 32));
-  if (!(temperature > 0.f) || top == -INFINITY) {
-    if (rank == 0 && tid == 0) a.out[row] = static_cast<int>(~static_cast<uint32_t>(best));
+  w.top = key_value(combine_max(w, order_key(top)));
+  if (!(w.temperature > 0.f) || w.top == -INFINITY) {
+    const int token = first_highest(w, V);
+    if (rank == 0 && tid == 0) a.out[row] = token;
     return;
   }
-  const double max = top, factor = 64.0 * 1.4426950408889634 / temperature;
+  if (w.top == INFINITY) {                               // infinite logits share all the weight
+    for (int i = 0; i < shape.run; ++i) w.own[i] = w.own[i] == INFINITY ? 0.f : -INFINITY;
+    w.top = 0.f;
+  }
+  w.max = w.top, w.factor = 64.0 * 1.4426950408889634 / w.temperature;
+  w.reach = 660.f * w.temperature;                       // distance beyond which a weight is 0
+  w.step = fminf(kPerUnit / w.temperature, 3e38f);
+  // in registers, unlike what calls see of the row
+  const float* const own = data + tid * shape.stride;
+  const float step = w.step, reach = w.reach;
+  const double max = w.max, factor = w.factor, least_weight = w.floor_w;
+  top = w.top;
   const int S = a.bits;
-  double floor_w = a.min_p ? static_cast<double>(a.min_p[row]) : 0.0;
-  floor_w = (floor_w > 1.0 ? 1.0 : floor_w) * static_cast<double>(1ull << S);
-  // the weight in units of 2^-S: 2^(k / 64) 2^(r / 64) with |r| <= 1/2, the second factor by its series up to r^4 (error 4e-14)
-  auto weight = [&](float x) -> double {
-    if (x == top) return static_cast<double>(1ull << S);
-    const double y = (static_cast<double>(x) - max) * factor;
-    if (!(y > -64.0 * 55)) return 0.0;                   // below 2^-55, or the NaN of infinities
-    const double t = y + kMagic, r = y - (t - kMagic);
-    const int k = __double2loint(t);
-    constexpr double b = 0.010830424696249145;           // ln 2 / 64
-    const double p = fma(r, fma(r, fma(r, fma(r, b * b * b * b / 24, b * b * b / 6), b * b / 2), b), 1.0);
-    const double v = sh.table[k & 63] * p;
-    return __hiloint2double(__double2hiint(v) + (((k >> 6) + S) << 20), __double2loint(v));
-  };
-  auto whole = [&](float x) -> unsigned long long {      // rounded: below 2^51
-    return static_cast<unsigned long long>(__double_as_longlong(weight(x) + 4503599627370496.0)) & 0xfffffffffffffull;
-  };
-  unsigned long long bound = 0;                          // tokens at or above it are kept
 
-  // ---- border by value: the first kept token, from the front of the order, at which the running mass reaches `target`
-  const float step = 64.f / temperature;
-  auto select = [&](auto mass_of, const bool weighted, unsigned long long target) -> unsigned long long {
-    // candidates: tokens of bin `bin` of the last division; of keys lo .. hi from the second one on
-    int level = 0, bin = 0, shift = 0;
-    uint32_t lo_key = 0, hi_key = 0xffffffffu;
-    auto first_bin = [&](float x) -> int {
-      const int b = static_cast<int>((top - x) * step);  // saturates; the NaN of infinities gives 0
-      return b < kBins - 1 ? b : kBins - 1;
-    };
-    auto candidate = [&](float x, uint32_t key) -> bool {        // before the division of this level
-      return level == 0 || (key >= lo_key && key <= hi_key && (level > 1 || first_bin(x) == bin));
-    };
-    for (;;) {
-      // divide
-      for (int i = tid; i < 3 * kBins; i += kRowThreads) (&sh.hist[0][0])[i] = 0;
-      __syncthreads();
-      each([&](float x, int i) {
-        const unsigned long long c = composite(x, i);
-        const uint32_t key = static_cast<uint32_t>(c >> 32);
-        if (c < bound || !candidate(x, key)) return;
-        const int b = level == 0 ? first_bin(x) : static_cast<int>((hi_key - key) >> shift);
-        if (!weighted) {
-          atomicAdd(&sh.hist[0][b], 1u);
-          return;
-        }
-        const unsigned long long m = mass_of(x);
-        const uint32_t m0 = m & 0xffff, m1 = (m >> 16) & 0xffff, m2 = static_cast<uint32_t>(m >> 32);
-        if (m0) atomicAdd(&sh.hist[0][b], m0);
-        if (m1) atomicAdd(&sh.hist[1][b], m1);
-        if (m2) atomicAdd(&sh.hist[2][b], m2);
-      });
-      sync();
-      // a CTA sums its share of the bins over the cluster, a thread a run of them
-      const int share = kBins / ranks, each_thread = (share + kRowThreads - 1) / kRowThreads;
-      unsigned long long h[4], sum = 0;
+  if (k >= V || k < 0) k = 0;
+  const bool nucleus = p < 1.f;
+  bool summed = false;                                   // the thread's kept weights are known without another pass
+  unsigned long long own_kept = 0;
+  if (k > 0 || nucleus) {
+    // ---- both borders at once.  A histogram of counts says in which bin the k-th token lies, and, as a bin's weights are alike to 0.8 %, between
+    // which bins the nucleus ends; one pass over the weights then sums what lies outside these bins exactly and lists their tokens.
+    const int last = k > 0 ? kBins : kBins - 1;          // what is in the last bin has no weight
+#pragma unroll 2
+    for (int i = 0; i < shape.run; i += 4) {
+      const float4 t = *reinterpret_cast<const float4*>(own + i);
+      const float v[4] = {t.x, t.y, t.z, t.w};
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        h[j] = 0;
-        const int b = tid * each_thread + j;
-        if (j < each_thread && b < share)
-          for (int r = 0; r < ranks; ++r) {
-            const uint32_t* from = ranks > 1 ? cluster.map_shared_rank(&sh.hist[0][0], r) : &sh.hist[0][0];
-            const int at = rank * share + b;
-            h[j] += from[at];
-            if (weighted) h[j] += (static_cast<unsigned long long>(from[kBins + at]) << 16) + (static_cast<unsigned long long>(from[2 * kBins + at]) << 32);
-          }
-        sum += h[j];
+        const int b = min_of(__float2int_ru((top - v[j]) * step), kBins - 1);
+        if (b < last) atomicAdd(&sh.hist[b >> 1], b & 1 ? 0x10000u : 1u);
       }
-      unsigned long long upto = sum;                     // inclusive over the CTA's threads
+    }
+    if (tid == 0) {
+      sh.bin_k = kBins, sh.left_k = sh.count_k = 0;
+      sh.bin_lo = sh.bin_hi = kBins;
+      sh.before_lo = sh.upto_hi = 0xffffffffu;
+    }
+    w.sync();
+    // a CTA adds up a share of the bins, a thread a run of up to four words of it, two bins each
+    const int share = kBins / 2 / ranks, words = max_of(share / kRowThreads, 1), word0 = rank * share + tid * words;
+    const bool busy = tid * words < share;
+    uint32_t* own_count = &sh.upper[0][0] + tid * words * 2;       // of the share's bins
+    int counted = 0;
+    float mass = 0.f, spread = 0.f;                      // by the bins' middles, and the variance of that for values anywhere in a bin
+    auto weight_of_bin = [&](int b) { return b == 0 ? 1.f : b < kBins - 1 ? fast_exp2(-1.4426950408889634f / kPerUnit * (b - 0.5f)) : 0.f; };
+    auto spread_of = [&](int b, int n, float g) {
+      // bf16 logits lie on a grid, so all of a bin may lie at one end of it: half its width for each; fp32: 1 / sqrt(12) of it, at random
+      const float e = g * (1.f / kPerUnit) * (sizeof(T) == 2 ? 0.51f * n : 0.29f), f = sizeof(T) == 2 ? e : e * e * n;
+      return b == 0 ? 0.f : f;
+    };
+#pragma unroll 1
+    for (int c = 0; c < words && busy; ++c) {
+      uint32_t y[8], lo = 0, hi = 0;
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const unsigned long long y = __shfl_up_sync(0xffffffffu, upto, o);
-        if (lane >= o) upto += y;
-      }
-      if (lane == 31) sh.scan[warp] = upto;
-      __syncthreads();
-      unsigned long long all = 0;
-      for (int w = 0; w < kRowWarps; ++w) {
-        if (w == warp) upto += all;
-        all += sh.scan[w];
-      }
-      if (tid < ranks) *cluster.map_shared_rank(&sh.parts[rank], tid) = all;
-      sync();
-      unsigned long long before = 0;
-      for (int r = 0; r < rank; ++r) before += sh.parts[r];
-      upto += before;
-      if (upto >= target && upto - sum < target) {       // one thread of the cluster
-        unsigned long long left = target - (upto - sum);
-        int b = rank * share + tid * each_thread;
+      for (int r = 0; r < 8; ++r) y[r] = r < ranks ? (ranks > 1 ? w.other(r) : &sh)->hist[word0 + c] : 0u;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          if (j + 1 < each_thread && left > h[j]) {
-            left -= h[j];
-            ++b;
-          } else {
+      for (int r = 0; r < 8; ++r) lo += y[r] & 0xffff, hi += y[r] >> 16;
+      own_count[2 * c] = lo, own_count[2 * c + 1] = hi;
+      counted += lo + hi;
+      const int b = 2 * (word0 + c);
+      const float g0 = weight_of_bin(b), g1 = weight_of_bin(b + 1);
+      mass += lo * g0 + hi * g1;
+      spread += spread_of(b, lo, g0) + spread_of(b + 1, hi, g1);
+    }
+    // running sums over the cluster's threads, inclusive, and the whole
+    int upto = warp_upto(counted);
+    float mass_up = warp_upto(mass), spread_up = warp_upto(spread), mass_all = 0.f, spread_all = 0.f;
+    __syncthreads();
+    if (lane == 31) sh.scan[warp][0] = upto, sh.scan[warp][1] = __float_as_uint(mass_up), sh.scan[warp][2] = __float_as_uint(spread_up);
+    __syncthreads();
+    int count_all = 0;
+#pragma unroll 4
+    for (int c = 0; c < kRowWarps; ++c) {
+      const int n = static_cast<int>(sh.scan[c][0]);
+      const float m = __uint_as_float(static_cast<uint32_t>(sh.scan[c][1])), e = __uint_as_float(static_cast<uint32_t>(sh.scan[c][2]));
+      if (c < warp) upto += n, mass_up += m, spread_up += e;
+      count_all += n, mass_all += m, spread_all += e;
+    }
+    if (ranks > 1) {
+      if (tid < ranks) {
+        unsigned long long* to = w.other(tid)->parts[w.turn][rank];
+        to[0] = count_all, to[1] = __float_as_uint(mass_all), to[2] = __float_as_uint(spread_all);
+      }
+      w.sync();
+      mass_all = spread_all = 0.f;
+#pragma unroll 1
+      for (int r = 0; r < ranks; ++r) {
+        const float m = __uint_as_float(static_cast<uint32_t>(sh.parts[w.turn][r][1])), e = __uint_as_float(static_cast<uint32_t>(sh.parts[w.turn][r][2]));
+        if (r < rank) upto += static_cast<int>(sh.parts[w.turn][r][0]), mass_up += m, spread_up += e;
+        mass_all += m, spread_all += e;
+      }
+      w.turn ^= 1;
+    }
+    int bin_k = kBins, left_k = 0, count_k = 0;          // bin of the k-th token, its place there, tokens there
+    if (k > 0) {
+      if (busy && upto >= k && upto - counted < k) {     // one thread of the cluster
+        int n = upto - counted;
+        float m = mass_up - mass, e = spread_up - spread;
+#pragma unroll 1
+        for (int c = 0; c < 2 * words; ++c) {
+          const int b = 2 * word0 + c, here = own_count[c];
+          const float g = weight_of_bin(b);
+          if (n + here >= k) {
+#pragma unroll 1
+            for (int r = 0; r < ranks; ++r) {
+              RowShared* to = w.other(r);
+              to->bin_k = b, to->left_k = k - n, to->count_k = here;
+              to->mass_k = m + (k - n) * g, to->spread_k = e + spread_of(b, k - n, g);
+            }
             break;
           }
-        }
-        for (int r = 0; r < ranks; ++r) {
-          RowShared* to = cluster.map_shared_rank(&sh, r);
-          to->found_key = b;
-          to->found_left = left;
-          to->list_size = 0;
-          to->lo_key = 0xffffffffu;
-          to->hi_key = 0;
+          n += here;
+          m += here * g, e += spread_of(b, here, g);
         }
       }
-      sync();
-      const int next_bin = static_cast<int>(sh.found_key);
-      target = sh.found_left;
-      // gather the bin
-      RowShared* lead = ranks > 1 ? cluster.map_shared_rank(&sh, 0) : &sh;
-      uint32_t least = 0xffffffffu, most = 0;
-      each([&](float x, int i) {
-        const unsigned long long c = composite(x, i);
-        const uint32_t key = static_cast<uint32_t>(c >> 32);
-        if (c < bound || !candidate(x, key) || (level == 0 ? first_bin(x) : static_cast<int>((hi_key - key) >> shift)) != next_bin) return;
-        const unsigned long long m = mass_of(x);
-        if (m == 0) return;
-        least = min(least, key);
-        most = key > most ? key : most;
-        const uint32_t at = atomicAdd(&lead->list_size, 1u);
-        if (at < kList) lead->list_key[at] = c, lead->list_mass[at] = m;
-      });
-      least = __reduce_min_sync(0xffffffffu, least);
-      most = __reduce_max_sync(0xffffffffu, most);
-      if (lane == 0 && most != 0) atomicMin(&lead->lo_key, least), atomicMax(&lead->hi_key, most);
-      sync();
-      const uint32_t size = lead->list_size;
-      if (size <= kList) {
-        if (rank == 0) {
-          // sort, then the first place at which the running mass reaches the target
-          int n = 32;
-          while (n < static_cast<int>(size)) n *= 2;
-          for (int i = size + tid; i < n; i += kRowThreads) sh.list_key[i] = 0, sh.list_mass[i] = 0;
-          __syncthreads();
-          for (int k = 2; k <= n; k *= 2)
-            for (int j = k / 2; j > 0; j /= 2) {
-              const int other = tid ^ j;
-              if (tid < n && other > tid) {
-                const unsigned long long x = sh.list_key[tid], y = sh.list_key[other];
-                if ((tid & k) == 0 ? x < y : x > y) {
-                  const unsigned long long mx = sh.list_mass[tid], my = sh.list_mass[other];
-                  sh.list_key[tid] = y, sh.list_key[other] = x;
-                  sh.list_mass[tid] = my, sh.list_mass[other] = mx;
-                }
-              }
-              __syncthreads();
+      w.sync();
+      bin_k = sh.bin_k, left_k = sh.left_k, count_k = sh.count_k;
+      mass_all = sh.mass_k, spread_all = sh.spread_k;
+    }
+    int bin_lo = kBins, bin_hi = kBins - 1;              // bins among which the nucleus ends
+    int listed = count_k;                                // tokens of the list
+    if (nucleus) {
+      auto off = [&](float m, float e) {
+        float root;
+        asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(root) : "f"(e));
+        return sizeof(T) == 2 ? e + 1e-5f * m : 5.f * root + 1e-4f * m;
+      };
+      const float goal = p * mass_all, wide = p * off(mass_all, spread_all);
+      if (busy && mass_up + off(mass_up, spread_up) + wide >= goal && !(mass_up - mass - off(mass_up - mass, spread_up - spread) - wide >= goal)) {
+        // two threads may both see the border between them: the lower bin counts, which has the fewer tokens too
+        int n = upto - counted;
+        float m = mass_up - mass, e = spread_up - spread;
+        bool lo = m + off(m, e) + wide >= goal, hi = m - off(m, e) - wide >= goal;
+#pragma unroll 1
+        for (int c = 0; c < 2 * words; ++c) {
+          const int b = 2 * word0 + c, here = own_count[c];
+          const float g = weight_of_bin(b);
+          m += here * g, e += spread_of(b, here, g);
+          const bool lo1 = m + off(m, e) + wide >= goal, hi1 = m - off(m, e) - wide >= goal;
+          const bool new_lo = lo1 && !lo, new_hi = hi1 && !hi;
+          if (new_lo || new_hi)
+#pragma unroll 1
+            for (int r = 0; r < ranks; ++r) {
+              RowShared* to = w.other(r);
+              if (new_lo) atomicMin(&to->bin_lo, static_cast<uint32_t>(b)), atomicMin(&to->before_lo, static_cast<uint32_t>(n));
+              if (new_hi) atomicMin(&to->bin_hi, static_cast<uint32_t>(b)), atomicMin(&to->upto_hi, static_cast<uint32_t>(n + here));
             }
-          unsigned long long m = tid < n ? sh.list_mass[tid] : 0, up = m;
-#pragma unroll
-          for (int o = 1; o < 32; o <<= 1) {
-            const unsigned long long y = __shfl_up_sync(0xffffffffu, up, o);
-            if (lane >= o) up += y;
-          }
-          if (lane == 31) sh.scan[warp] = up;
-          __syncthreads();
-          for (int w = 0; w < warp; ++w) up += sh.scan[w];
-          if (up >= target && up - m < target)
-            for (int r = 0; r < ranks; ++r) cluster.map_shared_rank(&sh, r)->found_key = sh.list_key[tid];
+          n += here;
+          lo = lo1, hi = hi1;
         }
-        sync();
-        return sh.found_key;
       }
-      const uint32_t least_all = lead->lo_key, most_all = lead->hi_key;
-      if (least_all == most_all) {                       // equal logits: so many of them, by token
-        const unsigned long long one = mass_of(key_value(least_all));
-        sh.found_left = (target + one - 1) / one;        // the same in all threads
-        lo_key = hi_key = least_all;
-        sync();                                          // nobody reads the list's words any more
-        return static_cast<unsigned long long>(least_all) << 32;
+      w.sync();
+      bin_lo = static_cast<int>(sh.bin_lo), bin_hi = static_cast<int>(sh.bin_hi);
+      const int before_lo = static_cast<int>(sh.before_lo), upto_hi = static_cast<int>(sh.upto_hi);
+      if (bin_lo == kBins || bin_hi == kBins || bin_hi < bin_lo) {
+        listed = bin_lo <= bin_k && bin_k < kBins ? k - left_k + count_k - before_lo : kList + 1;     // up to the k-th token's bin, or too many
+        bin_hi = min_of(bin_k, kBins - 2);
+      } else if (bin_hi >= bin_k) {
+        listed = k - left_k + count_k - before_lo;
+        bin_hi = min_of(bin_k, kBins - 2);
+      } else {
+        listed += upto_hi - before_lo;
       }
-      sync();
-      bin = next_bin;
-      lo_key = least_all, hi_key = most_all;
-      const int width = 32 - __clz(hi_key - lo_key);     // bits of the range
-      shift = width > 11 ? width - 11 : 0;
-      ++level;
     }
-  };
-  // ---- border by token: the first token at which the running mass reaches `target`; -1 in all threads but the one that owns it
-  auto locate = [&](auto mass_at, auto target_of) -> int {
-    unsigned long long sum = 0;
-    each([&](float x, int i) { sum += mass_at(x, i); });
-    unsigned long long upto = sum;
+    bool done = listed <= kList && (bin_lo <= bin_hi || !nucleus);
+    RowShared* lead = w.other(0);
+    // a bin's tokens are told by ceil(y) <= b where y <= b
+    const float y_lo = bin_lo - 1.f, y_hi = bin_hi, y_k = bin_k < kBins ? bin_k - 1.f : INFINITY, y_k1 = bin_k < kBins - 1 ? bin_k : INFINITY;
+    Sums sums = {{0, 0, 0}};                             // weights in front of the list's bins, and behind them up to the k-th token's
+    if (done) {
+      // All weights are added up; the tokens up to the list's bins, which are few in most rows, are looked at more closely.  32 tokens at a time:
+      // those for the list are noted in a mask and put there behind the 32.
+      unsigned long long all = 0, front = 0, list = 0;
+      const float y_near = nucleus ? fmaxf(y_hi, y_k1 < INFINITY ? y_k1 : 0.f) : y_k1;          // the last of them
+#pragma unroll 1
+      for (int base = 0; base < shape.run; base += 32) {
+        uint32_t noted = 0;
+        const int end = min_of(base + 32, shape.run);
+#pragma unroll 1
+        for (int i = base; i < end; i += 4) {
+          const float4 t = *reinterpret_cast<const float4*>(own + i);
+          const float v[4] = {t.x, t.y, t.z, t.w};
+          float y[4];
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const unsigned long long y = __shfl_up_sync(0xffffffffu, upto, o);
-      if (lane >= o) upto += y;
+          for (int j = 0; j < 4; ++j) y[j] = (top - v[j]) * step;
+          const bool near = fminf(fminf(y[0], y[1]), fminf(y[2], y[3])) <= y_near;
+          if (!near && !nucleus) continue;
+          double g[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) g[j] = weight_of(v[j], top, max, factor, reach, S, sh.table);
+          unsigned long long m[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) m[j] = Row::rounded(y[j] <= y_k1 ? g[j] : 0.0);
+          all += (m[0] + m[1]) + (m[2] + m[3]);
+          if (near) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const bool before = nucleus ? y[j] <= y_lo : y[j] <= y_k;
+              const bool in = !before && ((nucleus && y[j] <= y_hi) || (y[j] > y_k && y[j] <= y_k1));
+              if (before) front += m[j];
+              if (before && g[j] >= least_weight) own_kept += m[j];
+              if (in) list += m[j];
+              noted |= static_cast<uint32_t>(in) << (i - base + j);
+            }
+          }
+        }
+        if (__any_sync(0xffffffffu, noted)) {            // one addition to the list's size per warp
+          const int n = __popc(noted), upto_lane = warp_upto(n);
+          uint32_t at = 0;
+          if (lane == 31) at = atomicAdd(&lead->list_size, static_cast<uint32_t>(upto_lane));
+          at = __shfl_sync(0xffffffffu, at, 31) + upto_lane - n;
+#pragma unroll 1
+          for (; noted; noted &= noted - 1, ++at) {
+            const int i = base + __ffs(noted) - 1;
+            if (at < kList)
+              lead->list.key[at] = Row::composite(own[i], begin + tid * shape.run + i),
+              lead->list.mass[at] = Row::rounded(weight_of(own[i], top, max, factor, reach, S, sh.table));
+          }
+        }
+      }
+      sums.v[0] = front, sums.v[1] = all - front - list;
+      sums = combine(w, sums);
+      done = static_cast<int>(lead->list_size) <= kList;
     }
-    if (lane == 31) sh.scan[warp] = upto;
-    __syncthreads();
-    unsigned long long all = 0;
-    for (int w = 0; w < kRowWarps; ++w) {
-      if (w == warp) upto += all;
-      all += sh.scan[w];
+    auto goal_of = [&](unsigned long long sum) -> unsigned long long {
+      const double want = ceil(static_cast<double>(p) * static_cast<double>(sum));
+      return want > 1.0 ? static_cast<unsigned long long>(want) : 1ull;
+    };
+    if (done) {
+      const int size = static_cast<int>(lead->list_size);
+      if (rank > 0) {                                    // every CTA sorts a copy of the list
+#pragma unroll 1
+        for (int i = tid; i < size; i += kRowThreads) sh.list.key[i] = lead->list.key[i], sh.list.mass[i] = lead->list.mass[i];
+        __syncthreads();
+      }
+      sort_list(sh, size);
+      // of the list in order: the k-th token's bin keeps its first left_k
+      unsigned long long g[kOwnList], key[kOwnList];
+      bool at_k[kOwnList];
+      int before_k = 0;
+#pragma unroll
+      for (int j = 0; j < kOwnList; ++j) {
+        const int i = tid * kOwnList + j;
+        key[j] = i < size ? sh.sorted_key[i] : 0;
+        g[j] = i < size ? sh.sorted_mass[i] : 0;
+        at_k[j] = i < size && w.bin_of(key_value(static_cast<uint32_t>(key[j] >> 32))) == bin_k;
+        before_k += at_k[j];
+      }
+      int place = 0;
+      if (k > 0) {
+        int upk = static_cast<int>(run_up(sh, before_k).upto) - before_k;
+#pragma unroll
+        for (int j = 0; j < kOwnList; ++j) {
+          upk += at_k[j];
+          if (at_k[j] && upk == left_k) sh.found_left = tid * kOwnList + j;   // place of the k-th token in the list
+          if (at_k[j] && upk > left_k) g[j] = 0;
+        }
+        __syncthreads();
+        place = static_cast<int>(sh.found_left);
+      }
+      if (nucleus) {
+        unsigned long long sum = 0;
+#pragma unroll
+        for (int j = 0; j < kOwnList; ++j) sum += g[j];
+        const RunUp run_sum = run_up(sh, sum);
+        const unsigned long long front = sums.v[0], target = goal_of(front + sums.v[1] + run_sum.all);
+        const bool gap = sums.v[1] != 0;                 // weights between the bins and the k-th token's
+        // the border lies behind the front and among the list's first bins, or the bins were wrong
+        if (tid == 0) sh.found_key = kList;
+        __syncthreads();
+        unsigned long long up = front + run_sum.upto - sum;
+#pragma unroll
+        for (int j = 0; j < kOwnList; ++j) {
+          if (up < target && up + g[j] >= target && (!gap || w.bin_of(key_value(static_cast<uint32_t>(key[j] >> 32))) <= bin_hi))
+            sh.found_key = tid * kOwnList + j;
+          up += g[j];
+        }
+        __syncthreads();
+        place = static_cast<int>(sh.found_key);
+        done = place < kList && front < target;
+      }
+      if (done) {
+        w.set_edge(sh.sorted_key[place]);
+        // what is kept of the list, to its owners
+#pragma unroll 1
+        for (int i = tid; i <= place; i += kRowThreads) {
+          const int token = static_cast<int>(~static_cast<uint32_t>(sh.sorted_key[i])) - begin;
+          const unsigned long long m = sh.sorted_mass[i];
+          if (token >= 0 && token < shape.slice && m > 0 && w.weight(key_value(static_cast<uint32_t>(sh.sorted_key[i] >> 32))) >= w.floor_w)
+            atomicAdd(&sh.drawn[token / shape.run], m);
+        }
+        __syncthreads();
+        own_kept += sh.drawn[tid];
+        summed = true;
+      }
     }
-    if (tid < ranks) *cluster.map_shared_rank(&sh.parts[rank], tid) = all;
-    sync();
-    unsigned long long before = 0, total = 0;
-    for (int r = 0; r < ranks; ++r) {
-      if (r < rank) before += sh.parts[r];
-      total += sh.parts[r];
+    if (!done) {
+      // too many tokens in the list's bins, or the wrong bins: top-k first, then the nucleus of what it keeps
+#pragma unroll 1
+      for (int stage = k > 0 ? 0 : 1; stage < (nucleus ? 2 : 1); ++stage) {
+        unsigned long long target = left_k;
+        int from = bin_k, to = bin_k;
+        if (stage == 1) {
+          sums = sum_weights(w, y_lo, y_hi);
+          target = goal_of(sums.v[0] + sums.v[1] + sums.v[2]);
+          const bool inside = sums.v[0] < target && target <= sums.v[0] + sums.v[2];
+          if (inside) target -= sums.v[0];
+          from = inside ? bin_lo : 0, to = inside ? bin_hi : kBins - 1;
+        }
+        cut(w, stage == 0, target, from, to);
+      }
     }
-    const unsigned long long target = target_of(total);
-    upto += before;
-    if (!(upto >= target && upto - sum < target)) return -1;
-    unsigned long long left = target - (upto - sum);
-    for (int i = 0; i < shape.run; ++i) {
-      const unsigned long long m = mass_at(own[i], mine + i);
-      if (m >= left) return mine + i;
-      left -= m;
-    }
-    return -1;
-  };
-  // a border by value with its place among equal logits
-  auto cut = [&](auto mass_of, const bool weighted, unsigned long long target) {
-    const unsigned long long at = select(mass_of, weighted, target);
-    if (static_cast<uint32_t>(at) != 0) {                // a token's number is never 2^32 - 1
-      bound = at;
-      return;
-    }
-    const unsigned long long ties = sh.found_left;
-    __syncthreads();
-    const int token = locate(
-        [&](float x, int i) -> unsigned long long {
-          const unsigned long long c = composite(x, i);
-          return c >= bound && (c >> 32) == (at >> 32) ? 1ull : 0ull;
-        },
-        [&](unsigned long long total) { return ties < total ? ties : total; });
-    if (token >= 0)
-      for (int r = 0; r < ranks; ++r) cluster.map_shared_rank(&sh, r)->found_key = at | static_cast<uint32_t>(~token);
-    sync();
-    bound = sh.found_key;
-    sync();
-  };
-  const int k = a.top_k ? a.top_k[row] : 0;
-  if (k > 0 && k < V) cut([](float) -> unsigned long long { return 1; }, false, static_cast<unsigned long long>(k));
-  const float p = a.top_p ? a.top_p[row] : 1.f;
-  if (p < 1.f) {
-    unsigned long long sum = 0;
-    each([&](float x, int i) {
-      if (composite(x, i) >= bound) sum += whole(x);
-    });
-    const double want = ceil(static_cast<double>(p) * static_cast<double>(combine(sum, false)));
-    cut(whole, true, want > 1.0 ? static_cast<unsigned long long>(want) : 1ull);
   }
-  const float u = a.uniforms[row];
   const bool any = !(u > 0.f);                           // the first kept token of any weight, however small
-  const int token = locate(
-      [&](float x, int i) -> unsigned long long {
-        if (composite(x, i) < bound) return 0;
-        if (any && floor_w <= 0.0) return x == top || (static_cast<double>(x) - max) / temperature > -745.13 ? 1 : 0;
-        const double w = weight(x);
-        if (!(w >= floor_w)) return 0;
-        return any ? 1 : static_cast<unsigned long long>(__double_as_longlong(w + 4503599627370496.0)) & 0xfffffffffffffull;
-      },
-      [&](unsigned long long total) -> unsigned long long {
-        const unsigned long long t = any ? 1ull : static_cast<unsigned long long>(static_cast<double>(u) * static_cast<double>(total)) + 1;
-        return t < total ? t : total;
-      });
+  const int token = locate(w, any ? kAny : kWeights, 0.f, 0, u, summed && !any, own_kept);
   if (token >= 0) a.out[row] = token;
 }
 
@@ -598,11 +1070,16 @@ extern "C" int b200_sample_filtered(const void* logits, int64_t row_stride, int6
   SampleArgs a{logits, row_stride, vocab_size, uniforms, temperatures, top_k, top_p, min_p, out_tokens, 62};
   while ((1ll << (62 - a.bits)) < vocab_size) --a.bits;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
+  int sms = sm_count_cached();
+  if (sms <= 0) sms = 148;
+  // CTAs of a row: as many as let two of them fit an SM; more, down to 4,096 logits each, while one wave of CTAs takes all rows.  Times in us of 1,
+  // 2, 4 and 8 CTAs: 1 row of 32,000 29, 25, 21, 19; 16 of 32,000 33, 27, 23, 22; 64 of 32,000 38, 29, 29, 46; 256 of 32,000 84, 78, 99, 152;
+  // 512 of 8,000 45, 69, 117, 243; 8 of 4,000 17, 19, 19, 19; 32 of 131,072 with 4 and 8 78, 79.
   int ranks = 1;
   while (ranks < 8 && row_smem(vocab_size, ranks) > 110 * 1024) ranks *= 2;
-  while (ranks < 8 && num_rows * ranks * 2 <= 296 && vocab_size / ranks > 4096) ranks *= 2;
+  while (ranks < 8 && num_rows * ranks * 2 <= 2 * sms && vocab_size / ranks > 4096) ranks *= 2;
   if (row_smem(vocab_size, ranks) <= 226 * 1024 && row_shape(vocab_size, ranks).slice < 65536 && num_rows * ranks <= 2147483647) {
-    if (a.bits > 50) a.bits = 50;
+    if (a.bits > 45) a.bits = 45;                        // weights below e^-32 round to 0
     return dtype == B200_DTYPE_F32 ? launch_rows<float>(a, num_rows, ranks, s) : launch_rows<__nv_bfloat16>(a, num_rows, ranks, s);
   }
   const int grid = static_cast<int>(num_rows);
