@@ -836,19 +836,20 @@ int b200_sample_filtered(const void* logits, int64_t row_stride, int64_t num_row
                          const float* temperatures, const int32_t* top_k, const float* top_p, const float* min_p,
                          int64_t* out_tokens, int32_t dtype, void* stream);
 
-/* Pools that share page ids: pools [num_pools] holds their device addresses and page_bytes their bytes per page (device arrays).
+/* Pools that share page ids: pools [num_pools] holds their device addresses and page_bytes their bytes per page (device arrays),
+ * of which largest_page is the largest.
  * Page target[j] of every pool becomes page source[j]; pairs with a negative id are left out, ids outside the pool reported.  A pair
  * whose target is also a source of the call or the target of an earlier pair is not carried out and reported (B200_ERR_ARG). */
 size_t b200_copy_pages_workspace_bytes(int32_t num_pairs);
-int b200_copy_pages(const int64_t* pools, const int64_t* page_bytes, int32_t num_pools, int64_t num_pages, const int32_t* source,
-                    const int32_t* target, int32_t num_pairs, void* workspace, size_t workspace_bytes, int32_t* status,
+int b200_copy_pages(const int64_t* pools, const int64_t* page_bytes, int64_t largest_page, int32_t num_pools, int64_t num_pages,
+                    const int32_t* source, const int32_t* target, int32_t num_pairs, void* workspace, size_t workspace_bytes, int32_t* status,
                     void* stream);
 
 /* Moves the pages that block_tables [rows, width] names (negative entries name none) to the front of all pools: with L of them, those
  * with an id >= L go, in ascending order, to the unnamed ids < L, in ascending order; nothing else is written in the pools.
  * out_tables [rows, width] = the tables with the new ids, page_map [num_pages] = new id or -1, counts = {L, moves}; source and target
  * [num_pages] receive the moves.  Entries outside the pool are reported and become -1. */
-int b200_compact_pages(const int64_t* pools, const int64_t* page_bytes, int32_t num_pools, int64_t num_pages,
+int b200_compact_pages(const int64_t* pools, const int64_t* page_bytes, int64_t largest_page, int32_t num_pools, int64_t num_pages,
                        const int32_t* block_tables, int64_t bt_stride, int64_t rows, int32_t width, int32_t* out_tables,
                        int32_t* page_map, int32_t* source, int32_t* target, int32_t* counts, int32_t* status, void* stream);
 

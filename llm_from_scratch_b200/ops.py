@@ -1620,29 +1620,37 @@ def _on_current(dev: torch.device) -> None:
         raise ValueError(f"the tensors are on {dev}, which is not the current device")
 
 
-def _window_args(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor, num_seqs: int, window: int,
-                 first: int, out: torch.Tensor | None) -> torch.Tensor:
-    """Checks what both forms of the attention share; returns the output tensor."""
+def _window_pools(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor, num_seqs: int, window: int,
+                  first: int) -> tuple:
+    """Checks what both forms of the attention share; (tokens, Hq, D, num_blocks, block_size, Hkv, Dv, table width)."""
     if q.dim() != 3 or k_cache.dim() != 4 or v_cache.dim() != 4:
         raise ValueError("q must be [tokens, Hq, D] and the caches [num_blocks, block_size, Hkv, D]")
     T, Hq, D = q.shape
-    Hkv, Dv = k_cache.shape[2], v_cache.shape[3]
-    if k_cache.shape[3] != D or v_cache.shape[:3] != k_cache.shape[:3] or k_cache.dtype != q.dtype or v_cache.dtype != q.dtype:
+    nb, bs, Hkv, Dk = k_cache.shape
+    nv, bv, Hv, Dv = v_cache.shape
+    dtype = q.dtype
+    if Dk != D or nv != nb or bv != bs or Hv != Hkv or k_cache.dtype is not dtype or v_cache.dtype is not dtype:
         raise ValueError("cache shape/dtype does not match q")
     if Hkv == 0 or Hq % Hkv:
         raise ValueError("the query heads must be a multiple of the key heads")
     if not (k_cache.is_contiguous() and v_cache.is_contiguous()):
         raise ValueError("caches must be contiguous")
-    if block_tables.dtype != torch.int32 or block_tables.dim() != 2 or block_tables.shape[0] != num_seqs \
-            or (block_tables.shape[1] != 1 and block_tables.stride(1) != 1):
+    if block_tables.dim() != 2 or block_tables.dtype is not torch.int32:
+        raise ValueError("block_tables must be int32 [num_seqs, maxb]")
+    rows, width = block_tables.shape
+    if rows != num_seqs or (width != 1 and block_tables.stride(1) != 1):
         raise ValueError("block_tables must be int32 [num_seqs, maxb] with contiguous rows")
-    if num_seqs and block_tables.shape[1] == 0:
+    if num_seqs and width == 0:
         raise ValueError("block_tables must have a column")
-    if not 1 <= window <= 0x7FFFFFFF or not 0 <= first <= 0x7FFFFFFF:
+    if not (1 <= window <= 0x7FFFFFFF and 0 <= first <= 0x7FFFFFFF):
         raise ValueError("window must be at least 1 and first at least 0")
+    return T, Hq, D, nb, bs, Hkv, Dv, width
+
+
+def _window_out(q: torch.Tensor, shape: tuple, out: torch.Tensor | None) -> torch.Tensor:
     if out is None:
-        return torch.empty((T, Hq, Dv), dtype=q.dtype, device=q.device)
-    if out.shape != (T, Hq, Dv) or out.dtype != q.dtype or not out.is_contiguous():
+        return torch.empty(shape, dtype=q.dtype, device=q.device)
+    if out.shape != shape or out.dtype is not q.dtype or not out.is_contiguous():
         raise ValueError("out must be a contiguous [tokens, Hq, Dv] tensor of q's dtype")
     return out
 
@@ -1659,21 +1667,20 @@ def window_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     are (``out``).  Returns [tokens, Hq, Dv]."""
     dev = _cuda(q, k_cache, v_cache, block_tables, cu_seqlens_q, cu_seqlens_k, out)
     _on_current(dev)
+    entries = cu_seqlens_q.numel()
     for cu in (cu_seqlens_q, cu_seqlens_k):
-        if cu.dtype != torch.int32 or cu.dim() != 1 or not cu.is_contiguous() or cu.numel() != cu_seqlens_q.numel() or cu.numel() == 0:
+        if cu.dtype is not torch.int32 or cu.dim() != 1 or cu.numel() != entries or entries == 0 or not cu.is_contiguous():
             raise ValueError("cu_seqlens must be contiguous int32 tensors of num_seqs + 1 entries")
-    num_seqs = cu_seqlens_q.numel() - 1
-    out = _window_args(q, k_cache, v_cache, block_tables, num_seqs, window, first, out)
-    T, Hq, D = q.shape
-    nb, bs, Hkv, Dv = v_cache.shape
+    num_seqs = entries - 1
+    T, Hq, D, nb, bs, Hkv, Dv, width = _window_pools(q, k_cache, v_cache, block_tables, num_seqs, window, first)
+    out = _window_out(q, (T, Hq, Dv), out)
     if T and (q.stride(2) != 1 or (Hq > 1 and q.stride(1) != D)):
         raise ValueError("q heads must be contiguous")
     if max_seqlen_q < 0:
         raise ValueError("max_seqlen_q must not be negative")
     check(lib.b200_window_attention(q.data_ptr(), q.stride(0), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), T,
                                     cu_seqlens_q.data_ptr(), cu_seqlens_k.data_ptr(), num_seqs, min(int(max_seqlen_q), T), Hq, Hkv, D, Dv,
-                                    float(scale), block_tables.data_ptr(), block_tables.stride(0), block_tables.shape[1], bs, nb, int(window),
-                                    int(first),
+                                    scale, block_tables.data_ptr(), block_tables.stride(0), width, bs, nb, window, first,
                                     _dt(q), status_word(dev).data_ptr(), _stream()), "window_attention")
     return out
 
@@ -1684,16 +1691,15 @@ def window_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
     q: [B, Hq, D] contiguous.  Returns [B, Hq, Dv]; zeros for contexts without tokens."""
     dev = _cuda(q, k_cache, v_cache, block_tables, context_lens, out)
     _on_current(dev)
-    out = _window_args(q, k_cache, v_cache, block_tables, q.shape[0], window, first, out)
-    B, Hq, D = q.shape
-    nb, bs, Hkv, Dv = v_cache.shape
-    if context_lens.dtype != torch.int64 or context_lens.shape != (B,) or not context_lens.is_contiguous():
+    B, Hq, D, nb, bs, Hkv, Dv, width = _window_pools(q, k_cache, v_cache, block_tables, q.shape[0], window, first)
+    if context_lens.dtype is not torch.int64 or context_lens.dim() != 1 or context_lens.numel() != B or not context_lens.is_contiguous():
         raise ValueError("context_lens must be a contiguous int64 [B] tensor")
     if not q.is_contiguous():
         raise ValueError("q must be contiguous")
+    out = torch.empty_like(q) if out is None and Dv == D else _window_out(q, (B, Hq, Dv), out)
     check(lib.b200_window_decode(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), block_tables.data_ptr(),
-                                 block_tables.stride(0), block_tables.shape[1], context_lens.data_ptr(), B, Hq, Hkv, D, Dv, bs, nb, float(scale),
-                                 int(window), int(first), _dt(q), status_word(dev).data_ptr(), _stream()), "window_decode")
+                                 block_tables.stride(0), width, context_lens.data_ptr(), B, Hq, Hkv, D, Dv, bs, nb, scale,
+                                 window, first, _dt(q), status_word(dev).data_ptr(), _stream()), "window_decode")
     return out
 
 
@@ -1747,9 +1753,8 @@ class PagePools:
         addresses = [t.data_ptr() for t in self.tensors]
         page_bytes = [size(t) // self.num_pages if self.num_pages else 0 for t in self.tensors]
         self._table = torch.tensor([addresses, page_bytes], dtype=torch.int64).to(self.device)
-
-    def _pointers(self):
-        return self._table[0].data_ptr(), self._table[1].data_ptr(), len(self.tensors), self.num_pages
+        at = self._table.data_ptr()
+        self._args = at, at + 8 * len(self.tensors), max(page_bytes), len(self.tensors), self.num_pages
 
 
 def _page_ids(name: str, t: torch.Tensor) -> None:
@@ -1771,7 +1776,7 @@ def copy_pages(pools: PagePools, source: torch.Tensor, target: torch.Tensor) -> 
     n = source.numel()
     nbytes = lib.b200_copy_pages_workspace_bytes(n)
     scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-    check(lib.b200_copy_pages(*pools._pointers(), source.data_ptr(), target.data_ptr(), n, _ptr(scratch), nbytes,
+    check(lib.b200_copy_pages(*pools._args, source.data_ptr(), target.data_ptr(), n, _ptr(scratch), nbytes,
                               status_word(dev).data_ptr(), _stream()), "copy_pages")
 
 
@@ -1795,10 +1800,12 @@ def compact_pages(pools: PagePools, block_tables: torch.Tensor) -> CompactedPage
     stride = block_tables.stride(0) if rows > 1 else width
     if stride < width:
         raise ValueError("block_tables rows must not overlap")
+    n = pools.num_pages
     tables = torch.empty((rows, width), dtype=torch.int32, device=dev)
-    page_map, source, target = (torch.empty(pools.num_pages, dtype=torch.int32, device=dev) for _ in range(3))
+    page_map = torch.empty(n, dtype=torch.int32, device=dev)
     counts = torch.empty(2, dtype=torch.int32, device=dev)
-    check(lib.b200_compact_pages(*pools._pointers(), block_tables.data_ptr(), stride, rows, width, tables.data_ptr(), page_map.data_ptr(),
-                                 source.data_ptr(), target.data_ptr(), counts.data_ptr(), status_word(dev).data_ptr(), _stream()),
+    moves = torch.empty(2 * n, dtype=torch.int32, device=dev)
+    check(lib.b200_compact_pages(*pools._args, block_tables.data_ptr(), stride, rows, width, tables.data_ptr(), page_map.data_ptr(),
+                                 moves.data_ptr(), moves.data_ptr() + 4 * n, counts.data_ptr(), status_word(dev).data_ptr(), _stream()),
           "compact_pages")
     return CompactedPages(tables, page_map, counts)

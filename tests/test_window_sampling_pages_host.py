@@ -116,11 +116,11 @@ def test_argument_errors_of_the_library():
     smp = lambda **c: lib.b200_sample_filtered(*{**dict(logits=x, stride=9, rows=1, vocab=9, u=x, t=x, k=None, p=None, m=None, out=x, dtype=0, stream=None), **c}.values())
     assert smp(vocab=0) == smp(stride=8) == smp(u=None) == smp(t=None) == smp(out=None) == -1
     assert smp(dtype=3) == -3 and smp(rows=0) == 0 and smp(vocab=(1 << 24) + 1, stride=1 << 25) == smp(rows=1 << 31) == -8
-    cpy = lambda **c: lib.b200_copy_pages(*{**dict(pools=x, sizes=x, n=1, pages=5, source=x, target=x, pairs=2, ws=None, nbytes=0, status=None, stream=None), **c}.values())
+    cpy = lambda **c: lib.b200_copy_pages(*{**dict(pools=x, sizes=x, largest=64, n=1, pages=5, source=x, target=x, pairs=2, ws=None, nbytes=0, status=None, stream=None), **c}.values())
     assert cpy(pairs=-1) == cpy(source=None) == cpy(pools=None) == -1 and cpy(pairs=0) == cpy(n=0) == 0
     assert lib.b200_copy_pages_workspace_bytes(1024) == 0 and lib.b200_copy_pages_workspace_bytes(1025) == 4100
     assert cpy(pairs=1025) == cpy(pairs=1025, ws=x, nbytes=4099) == -5
-    cmp_ = lambda **c: lib.b200_compact_pages(*{**dict(pools=x, sizes=x, n=1, pages=5, bt=x, stride=2, rows=3, width=2, out=x, map=x, source=x, target=x, counts=x,
+    cmp_ = lambda **c: lib.b200_compact_pages(*{**dict(pools=x, sizes=x, largest=64, n=1, pages=5, bt=x, stride=2, rows=3, width=2, out=x, map=x, source=x, target=x, counts=x,
                                                        status=None, stream=None), **c}.values())
     assert cmp_(stride=1) == cmp_(bt=None) == cmp_(map=None) == cmp_(counts=None) == cmp_(rows=-1) == -1 and cmp_(pages=1 << 31) == -8
 
