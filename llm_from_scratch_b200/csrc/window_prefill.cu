@@ -29,22 +29,23 @@ namespace b200 {
 namespace {
 
 constexpr int BM = 128, BN = 64;
-constexpr int kThreads = 384;
 constexpr int Q_SLAB = BM * 128;           // 64 columns of 128 rows
 constexpr int K_SLAB = BN * 128;           // 64 columns of 64 keys
 constexpr float kRescaleThreshold = 8.f;   // log2 units
 
-template <int D>
+// NP: problems of a CTA
+template <int D, int NP>
 struct Lay {
+  static constexpr int kThreads = 128 + NP * 128;
   static constexpr int S = D / 64;
   static constexpr int Q_BYTES = S * Q_SLAB, K_BYTES = S * K_SLAB, STAGE = 2 * K_BYTES;
   static constexpr int NST = 4;
-  static constexpr int OFF_KV = 2 * Q_BYTES, OFF_BAR = OFF_KV + NST * STAGE;
+  static constexpr int OFF_KV = NP * Q_BYTES, OFF_BAR = OFF_KV + NST * STAGE;
   // as in prefill_umma2.cu
   static constexpr int Q_FULL = 0, K_FULL = 1, V_FULL = 1 + NST, QK_DONE = 1 + 2 * NST, PV_DONE = 1 + 4 * NST, P_READY = 1 + 6 * NST,
                        TURN = P_READY + 4, NUM_BARS = TURN + 8;
   static constexpr int SMEM = OFF_BAR + NUM_BARS * 8 + 32 + 1024;
-  static constexpr int TCOLS = 512;
+  static constexpr int TCOLS = NP * (128 + D) > 256 ? 512 : 256;
 };
 
 struct PromptArgs {
@@ -111,12 +112,12 @@ __device__ __noinline__ void plain_row(const WindowArgs& a, int seq, int64_t row
   for (int i = 0; i < N; ++i) op[i] = __float2bfloat16_rn(l == 0.f ? 0.f : o[i] / l);
 }
 
-template <int D>
-__global__ void __launch_bounds__(kThreads, 1)
+template <int D, int NP>
+__global__ void __launch_bounds__(Lay<D, NP>::kThreads, NP == 1 ? 2 : 1)
 window_prefill_kernel(const PromptArgs p, const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                       const __grid_constant__ CUtensorMap tm_v) {
-  using L = Lay<D>;
-  constexpr int NST = L::NST;
+  using L = Lay<D, NP>;
+  constexpr int NST = L::NST, kThreads = L::kThreads;
   const WindowArgs& a = p.w;
   extern __shared__ uint8_t smem_raw[];
   __shared__ int s_tile[2];
@@ -131,7 +132,7 @@ window_prefill_kernel(const PromptArgs p, const __grid_constant__ CUtensorMap tm
 
   if (warp == 0) {
     int seq = -1, tile = 0;
-    find_tile(a.cu_q, a.num_seqs, 2 * p.tokens, blockIdx.x / a.Hkv, &seq, &tile);
+    find_tile(a.cu_q, a.num_seqs, NP * p.tokens, blockIdx.x / a.Hkv, &seq, &tile);
     if (lane == 0) s_tile[0] = seq, s_tile[1] = tile, s_again = 0;
   } else if (tid == 32) {
     umma::mbar_init(bar(L::Q_FULL), 1);
@@ -153,9 +154,9 @@ window_prefill_kernel(const PromptArgs p, const __grid_constant__ CUtensorMap tm
   if (seq < 0) return;                       // uniform over the CTA, before any allocation
   const int q0 = a.cu_q[seq], q_len = a.cu_q[seq + 1] - q0, k_len = a.cu_k[seq + 1] - a.cu_k[seq];
   const int off = k_len - q_len;             // position of the first query (negative: queries without a key)
-  const int m0 = s_tile[1] * 2 * p.tokens;
+  const int m0 = s_tile[1] * NP * p.tokens;
   // tokens of the two problems; B may be empty
-  const int toks[2] = {min(p.tokens, q_len - m0), max(0, min(p.tokens, q_len - m0 - p.tokens))};
+  const int toks[2] = {min(p.tokens, q_len - m0), NP == 2 ? max(0, min(p.tokens, q_len - m0 - p.tokens)) : 0};
   const bool has_b = toks[1] > 0;
   const int pos0 = off + m0, last = pos0 + toks[0] + toks[1] - 1;     // positions of the CTA's first and last row
   // the walk: key tiles 0 .. nf - 1 (first tokens), then those from `start` on
@@ -235,7 +236,7 @@ window_prefill_kernel(const PromptArgs p, const __grid_constant__ CUtensorMap tm
   } else if (warp < 4) {
     // =============================== MMA issuers ===============================
     const int x = warp - 2;
-    if (lane == 0 && nt[x] > 0) {
+    if (x < NP && lane == 0 && nt[x] > 0) {
       const uint32_t idesc_qk = umma::instr_desc_bf16(BM, BN, false, false);
       const uint32_t idesc_pv = umma::instr_desc_bf16(BM, D, false, true);
       const int nx = nt[x];
@@ -495,22 +496,22 @@ bool make_map(CUtensorMap* m, const void* base, int64_t rows, int heads, int D, 
                 CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int D>
+template <int D, int NP>
 int launch(const PromptArgs& p, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, int64_t ctas, cudaStream_t s) {
-  using L = Lay<D>;
+  using L = Lay<D, NP>;
   static_assert(L::SMEM <= 227 * 1024, "shared memory budget");
   static bool configured[64] = {};             // racing threads set the same attribute
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64) return B200_ERR_UNSUPPORTED;
   if (!configured[dev]) {
-    if (cudaFuncSetAttribute(window_prefill_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::SMEM) != cudaSuccess) {
+    if (cudaFuncSetAttribute(window_prefill_kernel<D, NP>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::SMEM) != cudaSuccess) {
       cudaGetLastError();
       return B200_ERR_LAUNCH;
     }
     configured[dev] = true;
   }
-  window_prefill_kernel<D><<<static_cast<unsigned>(ctas), kThreads, L::SMEM, s>>>(p, tq, tk, tv);
+  window_prefill_kernel<D, NP><<<static_cast<unsigned>(ctas), L::kThreads, L::SMEM, s>>>(p, tq, tk, tv);
   return launch_result();
 }
 
@@ -525,14 +526,15 @@ int window_prefill_launch(const WindowArgs& a, int64_t total_q, cudaStream_t s) 
   if (rows <= 0 || rows > 2147483647LL) return B200_ERR_UNSUPPORTED;       // coordinates of a copy are 32-bit
   if (!aligned16(a.q) || a.q_stride % 8 != 0 || !aligned16(a.kc) || !aligned16(a.vc) || !aligned16(a.out)) return B200_ERR_UNSUPPORTED;
   PromptArgs p{a, G, BM / G, a.bs < BN ? a.bs : BN};
-  const int64_t ctas = (total_q / (2 * p.tokens) + a.num_seqs) * a.Hkv;     // tiles of all portions, the last of each perhaps short
+  const int problems = a.D == 64 ? 1 : 2;
+  const int64_t ctas = (total_q / (problems * p.tokens) + a.num_seqs) * a.Hkv;     // tiles of all portions, the last of each perhaps short
   if (ctas > 2147483647LL || a.num_seqs > (1 << 20)) return B200_ERR_UNSUPPORTED;
   CUtensorMap tq, tk, tv;
   if (!make_map(&tq, a.q, total_q, a.Hq, a.D, a.q_stride, G, p.tokens) ||
       !make_map(&tk, a.kc, rows, a.Hkv, a.D, static_cast<int64_t>(a.Hkv) * a.D, 1, p.box) ||
       !make_map(&tv, a.vc, rows, a.Hkv, a.D, static_cast<int64_t>(a.Hkv) * a.D, 1, p.box))
     return B200_ERR_UNSUPPORTED;
-  return a.D == 128 ? launch<128>(p, tq, tk, tv, ctas, s) : launch<64>(p, tq, tk, tv, ctas, s);
+  return a.D == 128 ? launch<128, 2>(p, tq, tk, tv, ctas, s) : launch<64, 1>(p, tq, tk, tv, ctas, s);
 }
 
 }  // namespace b200
