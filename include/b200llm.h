@@ -101,6 +101,8 @@ int64_t b200_pool_num_free(const void* pool);
 int64_t b200_pool_allocate(void* pool, const int32_t* token_ids_host, int64_t num_tokens, int32_t* table_out_host,
                            int64_t* num_cached_out_host);
 int b200_pool_deallocate(void* pool, const int32_t* table_host, int64_t num_blocks);
+/* One more sequence uses these blocks (all in use, else nothing is changed: B200_ERR_ARG). */
+int b200_pool_share(void* pool, const int32_t* table, int64_t num_blocks);
 int64_t b200_pool_append(void* pool, int32_t last_block, int32_t prev_block, int64_t num_tokens,
                          const int32_t* last_block_tokens_host);
 int64_t b200_pool_open_block(void* pool);

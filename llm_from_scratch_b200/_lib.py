@@ -32,6 +32,7 @@ SIGNATURES = {
     "b200_pool_num_free": (_i64, [_vp]),
     "b200_pool_allocate": (_i64, [_vp, _vp, _i64, _vp, _vp]),
     "b200_pool_deallocate": (_i32, [_vp, _vp, _i64]),
+    "b200_pool_share": (_i32, [_vp, _vp, _i64]),
     "b200_pool_append": (_i64, [_vp, _i32, _i32, _i64, _vp]),
     "b200_pool_open_block": (_i64, [_vp]),
     "b200_pool_seal_block": (_i32, [_vp, _i32, _i32, _vp]),

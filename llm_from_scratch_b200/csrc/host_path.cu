@@ -147,6 +147,16 @@ extern "C" int b200_pool_deallocate(void* pool, const int32_t* table, int64_t nu
   return B200_OK;
 }
 
+// One more sequence uses these blocks.
+extern "C" int b200_pool_share(void* pool, const int32_t* table, int64_t num_blocks) {
+  Pool* p = static_cast<Pool*>(pool);
+  if (!p || num_blocks < 0 || (num_blocks > 0 && !table)) return B200_ERR_ARG;
+  for (int64_t i = 0; i < num_blocks; ++i)
+    if (!b200::valid_block(p, table[i]) || p->ref[table[i]] <= 0) return B200_ERR_ARG;
+  for (int64_t i = 0; i < num_blocks; ++i) ++p->ref[table[i]];
+  return B200_OK;
+}
+
 // Decode-time growth for a sequence that has just reached `num_tokens` tokens (the call the scheduler makes
 // before each decode step), given the last block of its table and the one before it (-1: none): at
 // num_tokens % block_size == 1 a fresh block is opened and returned (>= 0); at == 0 the now full last block is

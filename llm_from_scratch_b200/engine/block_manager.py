@@ -186,13 +186,35 @@ class BlockManager:
 
     def deallocate(self, seq: Sequence) -> None:
         order = seq.block_table if self.reference_exact else reversed(seq.block_table)
-        for block_id in order:
+        self._give_back(order)
+        seq.block_table = []
+        seq.num_cached_tokens = 0
+
+    def _give_back(self, block_ids) -> None:
+        for block_id in block_ids:
+            if block_id < 0:                # given back earlier (``release``)
+                continue
             block = self.blocks[block_id]
             block.ref_count -= 1
             if block.ref_count == 0:
                 self._deallocate_block(block_id)
-        seq.block_table = []
-        seq.num_cached_tokens = 0
+
+    def release(self, seq: Sequence, start: int, end: int) -> None:
+        """Gives back blocks start .. end - 1 of ``seq``, which no later step reads; their entries become -1."""
+        if self.reference_exact:
+            raise ValueError("the reference's ref-count arithmetic does not give single blocks back")
+        self._give_back(reversed(seq.block_table[start:end]))
+        seq.block_table[start:end] = [-1] * (end - start)
+
+    def fork(self, seq: Sequence, child: Sequence) -> list[tuple[int, int]]:
+        """Gives ``child``, which continues from the tokens of ``seq``, its block table: full blocks are shared, those that the next
+        tokens are written to are opened anew.  Returns the (source, target) blocks to copy."""
+        if self.reference_exact:
+            raise ValueError("the reference's ref-count arithmetic has no forks")
+        return _fork(self, seq, child, lambda ids: [self._share(b) for b in ids])
+
+    def _share(self, block_id: int) -> None:
+        self.blocks[block_id].ref_count += 1
 
     # ------------------------------------------------------------------ decode-time growth
     def can_append(self, seq: Sequence) -> bool:
@@ -235,6 +257,20 @@ class BlockManager:
         block.update(h, token_ids)
         self.hash_to_block_id[h] = block.block_id
 
+
+
+def _fork(manager, seq: Sequence, child: Sequence, share) -> list[tuple[int, int]]:
+    bs, written = manager.block_size, seq.num_tokens - 1          # the last token's keys do not exist yet
+    full = min(written // bs, len(seq.block_table))
+    own = len(seq.block_table) - full                             # at most the open block and one opened ahead
+    if own > manager.num_free_blocks:
+        raise IndexError("KV block pool exhausted")
+    child.block_table = seq.block_table[:full]
+    share([b for b in child.block_table if b >= 0])
+    for _ in range(own):
+        manager.open_block(child)
+    child.num_cached_tokens = seq.num_cached_tokens
+    return [(seq.block_table[full], child.block_table[full])] if own and written % bs else []
 
 
 class _BlockView:
@@ -333,11 +369,28 @@ class NativeBlockManager:
         seq.num_cached_tokens += self._cached.value
 
     def deallocate(self, seq: Sequence) -> None:
-        table = self._np.asarray(seq.block_table, dtype=self._np.int32)
-        if self._lib.b200_pool_deallocate(self._h, table.ctypes.data, table.size) != 0:
-            raise RuntimeError("deallocate: a block of the table is not in use")
+        self._give_back(seq.block_table)
         seq.block_table = []
         seq.num_cached_tokens = 0
+
+    def _give_back(self, block_ids) -> None:
+        table = self._np.asarray(block_ids, dtype=self._np.int32)
+        table = table[table >= 0]           # -1: given back earlier (``release``)
+        if self._lib.b200_pool_deallocate(self._h, table.ctypes.data, table.size) != 0:
+            raise RuntimeError("deallocate: a block of the table is not in use")
+
+    def release(self, seq: Sequence, start: int, end: int) -> None:
+        """``BlockManager.release``."""
+        self._give_back(seq.block_table[start:end])
+        seq.block_table[start:end] = [-1] * (end - start)
+
+    def fork(self, seq: Sequence, child: Sequence) -> list[tuple[int, int]]:
+        """``BlockManager.fork``."""
+        def share(ids):
+            table = self._np.asarray(ids, dtype=self._np.int32)
+            if self._lib.b200_pool_share(self._h, table.ctypes.data, table.size) != 0:
+                raise RuntimeError("fork: a block of the table is not in use")
+        return _fork(self, seq, child, share)
 
     # ------------------------------------------------------------------ decode-time growth
     def can_append(self, seq: Sequence) -> bool:

@@ -35,6 +35,7 @@ class LLMEngine:
             self.scheduler = MixedScheduler(**limits, num_state_slots=self.model_runner.num_state_slots)
         else:
             self.scheduler = Scheduler(**limits)
+            self.scheduler.attention_cut = getattr(self.model_runner, "attention_cut", None)
         # decode steps the engine may run per scheduling decision (1 = the reference's step-by-step loop);
         # larger values keep the GPU busy while the host schedules, at the price of admitting waiting
         # requests and retiring finished ones up to decode_window - 1 steps later
@@ -62,6 +63,20 @@ class LLMEngine:
                 raise ValueError("a string prompt needs a tokenizer; pass token ids or LLMEngine(tokenizer=...)")
             prompt = self.tokenizer.encode(prompt)
         return self.add_request(prompt, sampling_params)
+
+    def fork(self, seq: Sequence, n: int = 1, sampling_params: SamplingParams | None = None) -> list[Sequence]:
+        """``n`` further continuations of a running sequence from the tokens it has now, under ``sampling_params`` (None: its own).
+        They share its full cache blocks; the block that is still being written is copied (``ops.copy_pages``).  Between two steps only."""
+        children, copies = [], []
+        try:
+            for _ in range(n):
+                child, pairs = self.scheduler.fork(seq, sampling_params)
+                children.append(child)
+                copies += pairs
+        finally:
+            if copies:
+                self.model_runner.copy_blocks(copies)
+        return children
 
     # ------------------------------------------------------------------ one step
     def step(self):

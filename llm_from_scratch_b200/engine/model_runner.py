@@ -107,6 +107,10 @@ class ModelRunner:
         # sliding windows of its layers: portions then need only the ends of their contexts
         self.attention_windows = tuple(getattr(model, "attention_windows", ()))
         self.attention_chunks = tuple(getattr(model, "attention_chunks", ()))     # the same for chunks of positions
+        # (window, first tokens) that bound what any layer sees of a context: pages between them can be given back
+        window = getattr(self.model_config, "attention_window", 0)
+        self.attention_cut = (window, self.model_config.attention_first) if window else None
+        self.page_pools = None
         self.num_state_slots = self.max_num_seqs if self.recurrent_state else 0
         if self.mixed_batches:      # their matrix products accumulate in fp32 from end to end
             torch.backends.cuda.matmul.allow_bf16_reduced_precision_reduction = False
@@ -234,7 +238,7 @@ class ModelRunner:
                                     chunk_ranges={c: key_range(f"chunk{c}", r) for c, r in parts.chunk_ranges.items()})
 
     def prepare_prefill(self, seqs: list[Sequence]) -> torch.Tensor:
-        return self._publish(md.prepare_prefill(seqs, self.block_size, tables_always=self.mixed_batches))
+        return self._publish(md.prepare_prefill(seqs, self.block_size, tables_always=self.mixed_batches or self.attention_cut is not None))
 
     def prepare_decode(self, seqs: list[Sequence]) -> torch.Tensor:
         return self._publish(md.prepare_decode(seqs, self.block_size))
@@ -244,6 +248,30 @@ class ModelRunner:
         if not any(temps):
             return None   # all greedy
         return torch.tensor(temps, dtype=torch.float32).to(self.device, non_blocking=True)
+
+    def prepare_filters(self, seqs: list[Sequence]) -> tuple:
+        """(top_k, top_p, min_p) of a batch that samples, each None where no row uses it."""
+        if not any(s.filters for s in seqs):
+            return None, None, None
+        rows = [s.filters or (0, 1.0, 0.0) for s in seqs]
+        columns = zip(*rows)
+        put = lambda values, off, dtype: None if all(v == off for v in values) else \
+            torch.tensor(values, dtype=dtype).to(self.device, non_blocking=True)
+        return tuple(put(c, off, dtype) for c, off, dtype in
+                     zip(columns, (0, 1.0, 0.0), (torch.int32, torch.float32, torch.float32)))
+
+    # ------------------------------------------------------------------ pages
+    def copy_blocks(self, pairs: list[tuple[int, int]]) -> None:
+        """Copies whole blocks (source, target) in all layers' pools, behind the steps queued so far."""
+        if not pairs:
+            return
+        if self.page_pools is None:
+            if self.layered_cache is not None:
+                raise ValueError("blocks of a model with layers of several kinds are not copied")
+            pools = self.kv_cache.flatten(0, 1) if self.kv_cache.dim() == 6 else self.kv_cache
+            self.page_pools = ops.PagePools(list(pools))
+        ids = torch.tensor(pairs, dtype=torch.int32).t().contiguous().to(self.device, non_blocking=True)
+        ops.copy_pages(self.page_pools, ids[0], ids[1])
 
     # ------------------------------------------------------------------ execution
     @torch.inference_mode()
@@ -293,7 +321,8 @@ class ModelRunner:
             if greedy:
                 token_ids = self.model.greedy_tokens(hidden).tolist()
             else:
-                token_ids = self.sampler(self.model.compute_logits(hidden), self.prepare_sample(seqs)).tolist()
+                token_ids = self.sampler(self.model.compute_logits(hidden), self.prepare_sample(seqs),
+                                         *self.prepare_filters(seqs)).tolist()
         reset_context()
         return token_ids
 

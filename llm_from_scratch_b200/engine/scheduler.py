@@ -34,6 +34,8 @@ class Scheduler:
         else:
             self.block_manager = NativeBlockManager(max_cached_blocks, block_size)
         self.state_slots = None       # StateSlots of a model with recurrent state (MixedScheduler)
+        # (window, first tokens) of a model none of whose layers sees more of a context: blocks between them are given back
+        self.attention_cut: tuple[int, int] | None = None
         self.waiting: deque[Sequence] = deque()
         self.running: deque[Sequence] = deque()
 
@@ -79,8 +81,23 @@ class Scheduler:
             if opening <= bm.num_free_blocks:
                 for s in edge:
                     bm.append(s)
+                    self._release_unseen(s)
                 return batch
         return self._grow_running_general(limit)
+
+    def _release_unseen(self, seq: Sequence) -> None:
+        """Gives back the blocks that the next token and all later ones see nothing of.  The block before the one that is written to
+        stays: the latter's hash is chained to its."""
+        if self.attention_cut is None:
+            return
+        window, first = self.attention_cut
+        table, bs = seq.block_table, self.block_manager.block_size
+        start, end = -(-first // bs), min((seq.num_tokens - window) // bs, (seq.num_tokens - 1) // bs - 1)
+        at = end
+        while at > start and table[at - 1] >= 0:
+            at -= 1
+        if at < end:
+            self.block_manager.release(seq, at, end)
 
     def _grow_running_general(self, limit: int) -> list[Sequence]:
         bm, batch = self.block_manager, []
@@ -120,6 +137,7 @@ class Scheduler:
                     self.running.appendleft(seq)
                 break
             bm.append(seq)
+            self._release_unseen(seq)
             batch.append(seq)
         if batch:
             self.running.extendleft(reversed(batch))
@@ -156,6 +174,7 @@ class Scheduler:
             return 1
         for s in opening:
             bm.open_block(s)
+            self._release_unseen(s)
         return k
 
     def postprocess_window(self, seqs: list[Sequence], steps: list[list[int]]) -> int:
@@ -183,6 +202,21 @@ class Scheduler:
                 if j < last and n % bs == 0:
                     bm.seal_block(seq, n // bs - 1)
         return kept
+
+    def fork(self, seq: Sequence, sampling_params=None) -> tuple[Sequence, list[tuple[int, int]]]:
+        """A running sequence that continues from the tokens of ``seq`` on its own (``sampling_params`` None: those of ``seq``); it
+        shares the full blocks.  Returns it and the (source, target) blocks to copy before the next step."""
+        if seq.status is not SequenceStatus.RUNNING or seq not in self.running:
+            raise ValueError("only a running sequence can be forked")
+        child = Sequence(seq.token_ids, sampling_params)
+        child.num_prompt_tokens = seq.num_prompt_tokens
+        if sampling_params is None:
+            for name in ("temperature", "max_tokens", "ignore_eos", "max_model_length", "filters"):
+                setattr(child, name, getattr(seq, name))
+        copies = self.block_manager.fork(seq, child)
+        child.status = SequenceStatus.RUNNING
+        self.running.append(child)
+        return child, copies
 
     def preempt(self, seq: Sequence) -> None:
         self.block_manager.deallocate(seq)
@@ -254,6 +288,9 @@ class MixedScheduler(Scheduler):
             self.state_slots.take(seq)
         seq.status = SequenceStatus.RUNNING
         self.running.append(seq)
+
+    def fork(self, seq: Sequence, sampling_params=None):
+        raise ValueError("sequences of models with mixed batches cannot be forked: their states are not in blocks")
 
     def _release(self, seq: Sequence) -> None:
         self.block_manager.deallocate(seq)

@@ -32,7 +32,7 @@ class Sequence:
 
     __slots__ = ("seq_id", "status", "token_ids", "last_token", "num_tokens", "num_prompt_tokens",
                  "num_cached_tokens", "block_table", "temperature", "max_tokens", "ignore_eos",
-                 "max_model_length", "state_slot", "step_end", "_bt_cache", "_row")
+                 "max_model_length", "filters", "state_slot", "step_end", "_bt_cache", "_row")
 
     def __init__(self, token_ids, sampling_params: SamplingParams | None = None):
         sp = sampling_params if sampling_params is not None else SamplingParams()
@@ -51,6 +51,7 @@ class Sequence:
         self.max_tokens = sp.max_tokens
         self.ignore_eos = sp.ignore_eos
         self.max_model_length = sp.max_model_length
+        self.filters = (sp.top_k, sp.top_p, sp.min_p) if sp.filtered else None     # None: all off
 
     def __len__(self) -> int:
         return self.num_tokens
@@ -112,6 +113,7 @@ class Sequence:
     def __setstate__(self, state):
         self.num_tokens, self.num_prompt_tokens, self.num_cached_tokens, self.block_table, payload = state
         self.state_slot, self.step_end = -1, None
+        self.filters = None
         self._bt_cache = None
         self._row = None
         self.token_ids = payload if self.num_tokens == self.num_prompt_tokens else [payload]

@@ -25,6 +25,8 @@ class ModelConfig:
     num_experts_per_tok: int = 1
     n_shared_experts: int = 1
     rms_eps: float = 1e-5                # RMSNorm of the residual stream (model/utils.py:49)
+    attention_window: int = 0            # GQA: tokens a token sees, itself included (0: all; the reference has no window)
+    attention_first: int = 0             # first tokens of a context that stay visible beside the window
 
     def __post_init__(self):
         if self.num_kv_heads is None:
@@ -35,6 +37,12 @@ class ModelConfig:
             raise ValueError(f"unsupported attention_type {self.attention_type!r}")
         if self.d_model % self.num_heads or self.num_heads % self.num_kv_heads:
             raise ValueError("d_model must divide by num_heads and num_heads by num_kv_heads")
+        if self.attention_window < 0 or self.attention_first < 0:
+            raise ValueError("attention_window and attention_first must not be negative")
+        if self.attention_window and self.attention_type != "GQA":
+            raise ValueError("attention_window needs GQA attention")
+        if self.attention_first and not self.attention_window:
+            raise ValueError("attention_first counts beside an attention_window")
 
     @property
     def head_dim(self) -> int:

@@ -291,6 +291,7 @@ class GQAAttention(nn.Module):
         self.rope = rope
         self.scale = self.hd ** -0.5
         self.dtype = p.dtype
+        self.window, self.first = cfg.attention_window, cfg.attention_first
         self.fused = True   # False: the same stage as separate tensor ops + store_kvcache
         # views into the pool; set by ModelRunner.allocate_kv_cache (model_runner.py:186-190)
         self.k_cache = self.v_cache = torch.empty(0)
@@ -311,7 +312,13 @@ class GQAAttention(nn.Module):
             k = apply_rope(k, positions, self.rope).to(self.dtype)
             if self.k_cache.numel():
                 ops.store_kvcache(k, v, self.k_cache, self.v_cache, ctx.slot_mapping)
-        if ctx.is_prefill:
+        if self.window:       # the step's own keys are in the pages as well
+            if ctx.is_prefill:
+                o = ops.window_attention(q, self.k_cache, self.v_cache, ctx.block_tables, ctx.cu_seqlens_q, ctx.cu_seqlens_k,
+                                         ctx.max_seqlen_q, self.scale, self.window, self.first, out=out)
+            else:
+                o = ops.window_decode(q, self.k_cache, self.v_cache, ctx.block_tables, ctx.context_lens, self.scale, self.window, self.first)
+        elif ctx.is_prefill:
             if ctx.block_tables is not None:   # part of the context is already cached
                 o = ops.prefill_varlen(q, None, None, ctx.cu_seqlens_q, ctx.cu_seqlens_k, ctx.max_seqlen_q,
                                        ctx.max_seqlen_k, self.scale, self.k_cache, self.v_cache, ctx.block_tables,
@@ -496,6 +503,8 @@ class EngineTransformerLM(TokenHead, nn.Module):
     def prefill_tile_rows(self) -> int:
         """Query rows per tile of the prefill kernel that serves this model (0: no tile list)."""
         c = self.cfg
+        if c.attention_window:           # its kernels find their tiles themselves
+            return 0
         if c.attention_type == "MLA":    # prefill runs the expanded form: 192-wide keys, 128-wide values
             return ops.prefill_tile_rows(c.num_heads, c.num_heads, c.head_dim + c.rope_dim, c.head_dim, self.dtype)
         return ops.prefill_tile_rows(c.num_heads, c.num_kv_heads, c.head_dim, c.head_dim, self.dtype)
