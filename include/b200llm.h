@@ -834,9 +834,10 @@ int b200_window_decode(const void* q, const void* k_cache, const void* v_cache, 
  * those the ones with w_i >= min_p; the draw is the first kept token, by number, at which the running sum of kept weights exceeds
  * u times their sum.  T <= 0 and rows without a logit above -inf: the first of the highest logits.  NaN counts as -inf.  The filter
  * arrays may be NULL (off).  vocab_size <= 2^24. */
+size_t b200_sample_filtered_workspace_bytes(int64_t num_rows, int32_t vocab_size);
 int b200_sample_filtered(const void* logits, int64_t row_stride, int64_t num_rows, int32_t vocab_size, const float* uniforms,
                          const float* temperatures, const int32_t* top_k, const float* top_p, const float* min_p,
-                         int64_t* out_tokens, int32_t dtype, void* stream);
+                         int64_t* out_tokens, void* workspace, size_t workspace_bytes, int32_t dtype, void* stream);
 
 /* Pools that share page ids: pools [num_pools] holds their device addresses and page_bytes their bytes per page (device arrays),
  * of which largest_page is the largest.

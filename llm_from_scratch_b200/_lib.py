@@ -132,7 +132,8 @@ SIGNATURES = {
                                      _i32, _i64, _i32, _i32, _i32, _vp, _vp]),
     "b200_window_decode": (_i32, [_vp, _vp, _vp, _vp, _vp, _i64, _i32, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _i64, _f32, _i32, _i32, _i32,
                                   _vp, _vp]),
-    "b200_sample_filtered": (_i32, [_vp, _i64, _i64, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _vp]),
+    "b200_sample_filtered_workspace_bytes": (_sz, [_i64, _i32]),
+    "b200_sample_filtered": (_i32, [_vp, _i64, _i64, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _i32, _vp]),
     "b200_copy_pages_workspace_bytes": (_sz, [_i32]),
     "b200_copy_pages": (_i32, [_vp, _vp, _i64, _i32, _i64, _vp, _vp, _i32, _vp, _sz, _vp, _vp]),
     "b200_compact_pages": (_i32, [_vp, _vp, _i64, _i32, _i64, _vp, _i64, _i64, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),

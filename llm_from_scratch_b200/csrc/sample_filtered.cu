@@ -19,36 +19,12 @@
 // Bound by the reads for large rows in principle; in fact by the weights (ten 64-bit operations each) and the histogram's additions.
 #include <cooperative_groups.h>
 
-#include <type_traits>
-
-#include "common.cuh"
+#include "sampling.cuh"
 
 namespace b200 {
 namespace {
 
 constexpr int kThreads = 512;
-
-struct SampleArgs {
-  const void* logits;
-  int64_t row_stride;
-  int vocab;
-  const float* uniforms;
-  const float* temperatures;
-  const int32_t* top_k;      // or null
-  const float* top_p;        // or null
-  const float* min_p;        // or null
-  int64_t* out;
-  int bits;                  // S
-};
-
-// Unsigned number with the order of the floats; NaN as -inf.
-__device__ __forceinline__ uint32_t order_key(float x) {
-  if (x != x) x = -INFINITY;
-  if (x == 0.f) x = 0.f;     // -0 and 0 are equal
-  const uint32_t b = __float_as_uint(x);
-  return b & 0x80000000u ? ~b : b | 0x80000000u;
-}
-__device__ __forceinline__ float key_value(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
 
 // ---------------------------------------------------------------------------------------------
 // rows that fit the shared memory of a cluster
@@ -58,7 +34,6 @@ constexpr int kBins = 4096, kOwnBins = kBins / kRowThreads;        // of the his
 constexpr int kSteps = 2048, kOwnSteps = kSteps / kRowThreads;     // of the histograms of weights
 constexpr int kList = 1024, kOwnList = kList / kRowThreads;        // tokens that are sorted at most
 constexpr float kPerUnit = 128.f;                                   // bins per distance T from the maximum: 32 T and the last bin
-constexpr double kMagic = 6755399441055744.0;                       // 1.5 * 2^52: added, it leaves the nearest whole number in the low bits
 
 struct alignas(16) RowShared {      // the logits lie behind it in 16-byte pieces
   double table[64];                  // 2^(i / 64)
@@ -99,39 +74,6 @@ __host__ __device__ inline RowShape row_shape(int vocab, int ranks) {
 }
 inline size_t row_smem(int vocab, int ranks) { return sizeof(RowShared) + static_cast<size_t>(kRowThreads) * row_shape(vocab, ranks).stride * 4; }
 
-__device__ __forceinline__ int min_of(int x, int y) { return x < y ? x : y; }
-__device__ __forceinline__ int max_of(int x, int y) { return x > y ? x : y; }
-
-// 2^(i / 64)
-__device__ const double kTable[64] = {
-    1.0, 1.0108892860517005, 1.0218971486541166, 1.0330248790212284,
-    1.0442737824274138, 1.0556451783605572, 1.0671404006768237, 1.0787607977571199,
-    1.0905077326652577, 1.102382583307841, 1.1143867425958924, 1.1265216186082418,
-    1.1387886347566916, 1.1511892299529827, 1.1637248587775775, 1.1763969916502812,
-    1.189207115002721, 1.202156731452703, 1.215247359980469, 1.22848053610687,
-    1.241857812073484, 1.255380757024691, 1.2690509571917332, 1.2828700160787783,
-    1.2968395546510096, 1.3109612115247644, 1.3252366431597413, 1.339667524053303,
-    1.3542555469368927, 1.3690024229745905, 1.383909881963832, 1.3989796725383112,
-    1.4142135623730951, 1.42961333839197, 1.4451808069770467, 1.460917794180647,
-    1.4768261459394993, 1.4929077282912648, 1.5091644275934228, 1.5255981507445384,
-    1.5422108254079407, 1.559004400237837, 1.5759808451078865, 1.593142151342267,
-    1.6104903319492543, 1.6280274218573478, 1.645755478153965, 1.6636765803267364,
-    1.681792830507429, 1.7001063537185235, 1.718619298122478, 1.7373338352737062,
-    1.7562521603732995, 1.7753764925265212, 1.7947090750031072, 1.8142521755003989,
-    1.8340080864093424, 1.8539791250833855, 1.8741676341103, 1.8945759815869656,
-    1.9152065613971474, 1.9360617934922943, 1.9571441241754002, 1.978456026387951};
-
-// The weight in units of 2^-S: 2^(n / 64) 2^(r / 64) with |r| <= 1/2, the second factor by its series up to r^4 (error 4e-14).
-__device__ __forceinline__ double weight_of(float x, float top, double max, double factor, float reach, int S, const double* table) {
-  const double y = (static_cast<double>(x) - max) * factor;
-  const double t = y + kMagic, r = y - (t - kMagic);
-  const int n = __double2loint(t);
-  constexpr double b = 0.010830424696249145;             // ln 2 / 64
-  const double q = fma(r, fma(r, fma(r, fma(r, b * b * b * b / 24, b * b * b / 6), b * b / 2), b), 1.0);
-  const double v = table[n & 63] * q;
-  return top - x > reach ? 0.0 : __hiloint2double(__double2hiint(v) + (((n >> 6) + S) << 20), __double2loint(v));
-}
-
 // What the kernel's parts know of a row.
 struct Row {
   RowShared* sh;
@@ -151,16 +93,9 @@ struct Row {
   }
   __device__ __forceinline__ bool kept(float x, int i) const { return x > edge || (x == edge && i <= edge_token); }
   __device__ __forceinline__ double weight(float x) const { return weight_of(x, top, max, factor, reach, S, sh->table); }
-  // below 2^51; 0 for weights below e^-32
-  static __device__ __forceinline__ unsigned long long rounded(double w) {
-    return static_cast<unsigned long long>(__double_as_longlong(w + 4503599627370496.0)) & 0xfffffffffffffull;
-  }
   // Bin 0: the maximum; bin b: distances above (b - 1) / 128 and up to b / 128 times T; the last one: all beyond, whose weights round to 0.
   __device__ __forceinline__ int bin_of(float x) const {               // never falls as x falls
     return min_of(__float2int_ru((top - x) * step), kBins - 1);      // saturates
-  }
-  static __device__ __forceinline__ unsigned long long composite(float x, int i) {
-    return static_cast<unsigned long long>(order_key(x)) << 32 | static_cast<uint32_t>(~i);
   }
   __device__ __forceinline__ void set_edge(unsigned long long c) {
     edge = key_value(static_cast<uint32_t>(c >> 32));
@@ -176,24 +111,6 @@ struct Row {
     }
   }
 };
-
-// Sum over the warp, in all lanes: three parts of 24 bits, whose sums fit 32.
-__device__ __forceinline__ unsigned long long warp_total(unsigned long long v) {
-  const uint32_t lo = __reduce_add_sync(0xffffffffu, static_cast<uint32_t>(v) & 0xffffffu);
-  const uint32_t mid = __reduce_add_sync(0xffffffffu, static_cast<uint32_t>(v >> 24) & 0xffffffu);
-  const uint32_t hi = __reduce_add_sync(0xffffffffu, static_cast<uint32_t>(v >> 48));
-  return lo + (static_cast<unsigned long long>(mid) << 24) + (static_cast<unsigned long long>(hi) << 48);
-}
-template <typename U>
-__device__ __forceinline__ U warp_upto(U v) {            // inclusive running sum over the lanes
-  const int lane = threadIdx.x & 31;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const U y = __shfl_up_sync(0xffffffffu, v, o);
-    if (lane >= o) v += y;
-  }
-  return v;
-}
 
 // A row's kernel runs through most of its code once, so fetching instructions sets the pace of small rows: of the stalls of one row of 32,000 more
 // than half are for instructions.  Calls out of line do not help, as they put the row's values into memory (256 rows of 131,072: 435 us
@@ -214,20 +131,6 @@ __device__ __noinline__ RunUp run_up(RowShared& sh, unsigned long long v) {
   return {warp > 0 ? v + before : v, __shfl_sync(0xffffffffu, upto, kRowWarps - 1)};
 }
 
-// Sorts the list into sorted_key / sorted_mass: a token's place is the number of those before it.
-__device__ __forceinline__ void sort_list(RowShared& sh, int size) {
-#pragma unroll 1
-  for (int i = threadIdx.x; i < size; i += kRowThreads) {
-    const unsigned long long key = sh.list.key[i];
-    int place = 0;
-#pragma unroll 4
-    for (int j = 0; j < size; ++j) place += sh.list.key[j] > key;
-    sh.sorted_key[place] = key;
-    sh.sorted_mass[place] = sh.list.mass[i];
-  }
-  __syncthreads();
-}
-
 // What the tokens of a group of four add to a running mass: ones for kept tokens equal to `x0`; or kept weights above the floor; or ones for kept
 // tokens of any weight above the floor.
 enum Mass { kTies, kWeights, kAny };
@@ -242,7 +145,7 @@ __device__ __forceinline__ void mass_of_four(const Row& w, Mass kind, float x0, 
     const bool counts = in[j] && g >= w.floor_w;
     if (kind == kTies) m[j] = in[j] && v[j] == x0;
     else if (kind == kAny) m[j] = counts && static_cast<double>(v[j]) - w.max > -745.13 * w.temperature;
-    else m[j] = counts ? Row::rounded(g) : 0ull;
+    else m[j] = counts ? rounded(g) : 0ull;
   }
 }
 
@@ -323,7 +226,7 @@ __device__ __forceinline__ void cut(Row& w, const bool ones, unsigned long long 
     }
     return s >= 0 && w.kept(x, i) ? s : -1;
   };
-  auto mass_of = [&](float x) -> unsigned long long { return ones ? 1ull : Row::rounded(w.weight(x)); };
+  auto mass_of = [&](float x) -> unsigned long long { return ones ? 1ull : rounded(w.weight(x)); };
   for (;;) {
     w.sync();                                            // the list of an earlier use has been read
     for (int i = tid; i < kSteps; i += kRowThreads) sh.hist[i] = sh.upper[0][i] = sh.upper[1][i] = 0;
@@ -382,7 +285,7 @@ __device__ __forceinline__ void cut(Row& w, const bool ones, unsigned long long 
       const uint32_t key = order_key(x), at = atomicAdd(&lead->list_size, 1u);
       least = min(least, key);
       most = key > most ? key : most;
-      if (at < kList) lead->list.key[at] = Row::composite(x, w.mine + i), lead->list.mass[at] = m;
+      if (at < kList) lead->list.key[at] = composite(x, w.mine + i), lead->list.mass[at] = m;
     }
     least = __reduce_min_sync(0xffffffffu, least);
     most = __reduce_max_sync(0xffffffffu, most);
@@ -392,7 +295,8 @@ __device__ __forceinline__ void cut(Row& w, const bool ones, unsigned long long 
     const uint32_t least_all = lead->lo_key, most_all = lead->hi_key;
     if (size <= kList) {
       if (w.rank == 0) {
-        sort_list(sh, size);
+        for (int i = tid; i < size; i += kRowThreads) sh.sorted_key[i] = sh.list.key[i], sh.sorted_mass[i] = sh.list.mass[i];
+        sort_by_key<kRowThreads>(sh.sorted_key, sh.sorted_mass, size);
         unsigned long long m[kOwnList], own_sum = 0;
 #pragma unroll
         for (int j = 0; j < kOwnList; ++j) {
@@ -486,7 +390,7 @@ __device__ __forceinline__ Sums sum_weights(Row& w, const float y_lo, const floa
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const float y = (w.top - v[j]) * w.step;
-      if (w.kept(v[j], i + j)) s.v[y <= y_lo ? 0 : y <= y_hi ? 2 : 1] += Row::rounded(w.weight(v[j]));
+      if (w.kept(v[j], i + j)) s.v[y <= y_lo ? 0 : y <= y_hi ? 2 : 1] += rounded(w.weight(v[j]));
     }
   });
   return combine(w, s);
@@ -504,15 +408,14 @@ __device__ __forceinline__ int first_highest(Row& w, int vocab) {
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kRowThreads, 2) sample_row_kernel(const SampleArgs a) {
-  extern __shared__ __align__(16) uint8_t smem[];
+__device__ __forceinline__ void sample_row(const SampleArgs& a, const int row, uint8_t* smem) {
   RowShared& sh = *reinterpret_cast<RowShared*>(smem);
   float* data = reinterpret_cast<float*>(smem + sizeof(RowShared));
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, V = a.vocab;
   Row w;
   w.sh = &sh;
   w.rank = cooperative_groups::this_cluster().block_rank(), w.ranks = cooperative_groups::this_cluster().num_blocks();
-  const int row = blockIdx.x / w.ranks, rank = w.rank, ranks = w.ranks;
+  const int rank = w.rank, ranks = w.ranks;
   w.shape = row_shape(V, ranks);
   const RowShape shape = w.shape;
   const int begin = rank * shape.slice;
@@ -778,7 +681,7 @@ __global__ void __launch_bounds__(kRowThreads, 2) sample_row_kernel(const Sample
           for (int j = 0; j < 4; ++j) g[j] = weight_of(v[j], top, max, factor, reach, S, sh.table);
           unsigned long long m[4];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) m[j] = Row::rounded(y[j] <= y_k1 ? g[j] : 0.0);
+          for (int j = 0; j < 4; ++j) m[j] = rounded(y[j] <= y_k1 ? g[j] : 0.0);
           all += (m[0] + m[1]) + (m[2] + m[3]);
           if (near) {
 #pragma unroll
@@ -801,8 +704,8 @@ __global__ void __launch_bounds__(kRowThreads, 2) sample_row_kernel(const Sample
           for (; noted; noted &= noted - 1, ++at) {
             const int i = base + __ffs(noted) - 1;
             if (at < kList)
-              lead->list.key[at] = Row::composite(own[i], begin + tid * shape.run + i),
-              lead->list.mass[at] = Row::rounded(weight_of(own[i], top, max, factor, reach, S, sh.table));
+              lead->list.key[at] = composite(own[i], begin + tid * shape.run + i),
+              lead->list.mass[at] = rounded(weight_of(own[i], top, max, factor, reach, S, sh.table));
           }
         }
       }
@@ -816,12 +719,10 @@ __global__ void __launch_bounds__(kRowThreads, 2) sample_row_kernel(const Sample
     };
     if (done) {
       const int size = static_cast<int>(lead->list_size);
-      if (rank > 0) {                                    // every CTA sorts a copy of the list
+      // every CTA sorts a copy of the list
 #pragma unroll 1
-        for (int i = tid; i < size; i += kRowThreads) sh.list.key[i] = lead->list.key[i], sh.list.mass[i] = lead->list.mass[i];
-        __syncthreads();
-      }
-      sort_list(sh, size);
+      for (int i = tid; i < size; i += kRowThreads) sh.sorted_key[i] = lead->list.key[i], sh.sorted_mass[i] = lead->list.mass[i];
+      sort_by_key<kRowThreads>(sh.sorted_key, sh.sorted_mass, size);
       // of the list in order: the k-th token's bin keeps its first left_k
       unsigned long long g[kOwnList], key[kOwnList];
       bool at_k[kOwnList];
@@ -904,8 +805,20 @@ __global__ void __launch_bounds__(kRowThreads, 2) sample_row_kernel(const Sample
   if (token >= 0) a.out[row] = token;
 }
 
+// A cluster per row; or, with a list of rows (their number first), a few clusters that walk it.
 template <typename T>
-int launch_rows(const SampleArgs& a, int64_t rows, int ranks, cudaStream_t s) {
+__global__ void __launch_bounds__(kRowThreads, 2) sample_row_kernel(const SampleArgs a, const int32_t* list) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  const int ranks = cooperative_groups::this_cluster().num_blocks(), first = blockIdx.x / ranks;
+  if (list == nullptr) return sample_row<T>(a, first, smem);
+  for (int i = first; i < list[0]; i += gridDim.x / ranks) {
+    sample_row<T>(a, list[1 + i], smem);
+    cooperative_groups::this_cluster().sync();           // the row's shared memory is used again
+  }
+}
+
+template <typename T>
+int launch_rows(const SampleArgs& a, int64_t rows, int ranks, const int32_t* list, cudaStream_t s) {
   static bool configured[64] = {};                       // racing threads set the same attribute
   int dev = 0;
   cudaGetDevice(&dev);
@@ -928,7 +841,7 @@ int launch_rows(const SampleArgs& a, int64_t rows, int ranks, cudaStream_t s) {
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return launch_result(cudaLaunchKernelEx(&cfg, sample_row_kernel<T>, a));
+  return launch_result(cudaLaunchKernelEx(&cfg, sample_row_kernel<T>, a, list));
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -1055,32 +968,56 @@ __global__ void __launch_bounds__(kThreads) sample_filtered_kernel(const SampleA
   if (tid == 0) a.out[row] = static_cast<int>(~static_cast<uint32_t>(at));
 }
 
+bool fits_cluster(int vocab) { return row_smem(vocab, 8) <= 226 * 1024 && row_shape(vocab, 8).slice < 65536; }
+
+// Whether passes of separate launches are faster than clusters.
+bool wide_is_faster(int64_t rows, int vocab) {
+  return fits_cluster(vocab) && sample_wide_takes(rows, vocab) && vocab >= 16384 && rows * vocab >= (int64_t(1) << 22);
+}
+
 }  // namespace
 }  // namespace b200
 
+extern "C" size_t b200_sample_filtered_workspace_bytes(int64_t num_rows, int32_t vocab_size) {
+  using namespace b200;
+  if (num_rows <= 0 || vocab_size <= 0) return 0;
+  return wide_is_faster(num_rows, vocab_size) ? sample_wide_workspace_bytes(num_rows, vocab_size) : 0;
+}
+
 extern "C" int b200_sample_filtered(const void* logits, int64_t row_stride, int64_t num_rows, int32_t vocab_size,
                                     const float* uniforms, const float* temperatures, const int32_t* top_k, const float* top_p,
-                                    const float* min_p, int64_t* out_tokens, int32_t dtype, void* stream) {
+                                    const float* min_p, int64_t* out_tokens, void* workspace, size_t workspace_bytes, int32_t dtype,
+                                    void* stream) {
   using namespace b200;
   if (num_rows < 0 || vocab_size <= 0 || row_stride < vocab_size) return B200_ERR_ARG;
   if (dtype != B200_DTYPE_F32 && dtype != B200_DTYPE_BF16) return B200_ERR_UNSUPPORTED;
   if (num_rows == 0) return B200_OK;
   if (!logits || !uniforms || !temperatures || !out_tokens) return B200_ERR_ARG;
   if (num_rows > 2147483647 || vocab_size > (1 << 24)) return B200_ERR_TOO_LARGE;
+  const size_t needed = b200_sample_filtered_workspace_bytes(num_rows, vocab_size);
+  if (needed > 0 && (!workspace || workspace_bytes < needed)) return B200_ERR_WORKSPACE;
   SampleArgs a{logits, row_stride, vocab_size, uniforms, temperatures, top_k, top_p, min_p, out_tokens, 62};
   while ((1ll << (62 - a.bits)) < vocab_size) --a.bits;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   int sms = sm_count_cached();
   if (sms <= 0) sms = 148;
-  // CTAs of a row: as many as let two of them fit an SM; more, down to 4,096 logits each, while one wave of CTAs takes all rows.  Times in us of 1,
-  // 2, 4 and 8 CTAs: 1 row of 32,000 29, 25, 21, 19; 16 of 32,000 33, 27, 23, 22; 64 of 32,000 38, 29, 29, 46; 256 of 32,000 84, 78, 99, 152;
-  // 512 of 8,000 45, 69, 117, 243; 8 of 4,000 17, 19, 19, 19; 32 of 131,072 with 4 and 8 78, 79.
-  int ranks = 1;
-  while (ranks < 8 && row_smem(vocab_size, ranks) > 110 * 1024) ranks *= 2;
-  while (ranks < 8 && num_rows * ranks * 2 <= 2 * sms && vocab_size / ranks > 4096) ranks *= 2;
-  if (row_smem(vocab_size, ranks) <= 226 * 1024 && row_shape(vocab_size, ranks).slice < 65536 && num_rows * ranks <= 2147483647) {
+  if (fits_cluster(vocab_size)) {
     if (a.bits > 45) a.bits = 45;                        // weights below e^-32 round to 0
-    return dtype == B200_DTYPE_F32 ? launch_rows<float>(a, num_rows, ranks, s) : launch_rows<__nv_bfloat16>(a, num_rows, ranks, s);
+    const int32_t* list = nullptr;
+    int64_t rows = num_rows;
+    // CTAs of a row: as many as let two of them fit an SM; more, down to 4,096 logits each, while one wave of CTAs takes all rows.  Times in us of
+    // 1, 2, 4 and 8 CTAs: 1 row of 32,000 29, 25, 21, 19; 16 of 32,000 33, 27, 23, 22; 64 of 32,000 38, 29, 29, 46; 256 of 32,000 84, 78, 99,
+    // 152; 512 of 8,000 45, 69, 117, 243; 8 of 4,000 17, 19, 19, 19; 32 of 131,072 with 4 and 8 78, 79.
+    int ranks = 1;
+    while (ranks < 8 && row_smem(vocab_size, ranks) > 110 * 1024) ranks *= 2;
+    while (ranks < 8 && num_rows * ranks * 2 <= 2 * sms && vocab_size / ranks > 4096) ranks *= 2;
+    if (needed > 0) {
+      const int rc = sample_wide_launch(a, num_rows, dtype, workspace, &list, s);
+      if (rc != B200_OK) return rc;
+      rows = 2 * sms / ranks;                            // clusters that walk the list, most often empty
+    }
+    if (rows * ranks <= 2147483647)
+      return dtype == B200_DTYPE_F32 ? launch_rows<float>(a, rows, ranks, list, s) : launch_rows<__nv_bfloat16>(a, rows, ranks, list, s);
   }
   const int grid = static_cast<int>(num_rows);
   if (dtype == B200_DTYPE_F32) sample_filtered_kernel<float><<<grid, kThreads, 0, s>>>(a);

@@ -1726,8 +1726,11 @@ def sample_filtered(logits: torch.Tensor, uniforms: torch.Tensor, temperatures: 
         out = torch.empty(B, dtype=torch.int64, device=logits.device)
     elif out.dtype != torch.int64 or out.numel() != B or not out.is_contiguous():
         raise ValueError("out must be contiguous int64 [B]")
+    nbytes = lib.b200_sample_filtered_workspace_bytes(B, V)
+    scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
     check(lib.b200_sample_filtered(logits.data_ptr(), logits.stride(0) if B > 1 else V, B, V, uniforms.data_ptr(), temperatures.data_ptr(),
-                                   _ptr(top_k), _ptr(top_p), _ptr(min_p), out.data_ptr(), _dt(logits), _stream()), "sample_filtered")
+                                   _ptr(top_k), _ptr(top_p), _ptr(min_p), out.data_ptr(), _ptr(scratch), nbytes, _dt(logits), _stream()),
+          "sample_filtered")
     return out
 
 

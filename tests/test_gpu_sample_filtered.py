@@ -164,3 +164,77 @@ def test_captured_and_on_two_streams():
                 g.replay()
     torch.cuda.synchronize()
     assert all(torch.equal(out, w) for _, out, w, _ in graphs)
+
+
+# ------------------------------------------------------------------------------------------------ many long rows: passes of separate launches
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,vocab,most,spread", [(130, 33000, 1000, (0.5, 8.0)), (260, 16384, 16384, (0.5, 8.0)), (33, 131072, 50000, (0.05, 3.0)),
+                                                 (45, 100001, 60, (1.0, 12.0))])
+def test_many_long_rows(n, vocab, most, spread, dtype):
+    from llm_from_scratch_b200._lib import lib
+    assert lib.b200_sample_filtered_workspace_bytes(n, vocab) > 0
+    x, u, t, g = rows(n, vocab, dtype, vocab, spread)
+    k, p, m = filters(n, vocab, g, most)
+    t[3], u[5] = 0.0, 0.0
+    for kk, pp, mm in ((k, p, m), (k, None, None), (None, p, None), (None, None, m), (None, None, None)):
+        assert torch.equal(call(x, u, t, kk, pp, mm), expect(x, u, t, kk, pp, mm))
+    p = torch.where(torch.arange(n) % 2 == 0, torch.full((n,), 0.995), torch.full((n,), 1e-3))
+    assert torch.equal(call(x, u, t, None, p, None), expect(x, u, t, None, p, None))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_edges_of_the_numbers_in_many_long_rows(dtype):
+    """What one form leaves to the other, between rows that it takes: greedy, masked, infinite, equal and flat rows."""
+    inf, nan = math.inf, math.nan
+    vocab, n = 66000, 66
+    x, u, t, g = rows(n, vocab, dtype, 3)
+    x[0] = -inf
+    x[1] = nan
+    x[2, ::2] = -inf
+    x[3, 1::2] = nan
+    x[4, [3, 50007]] = inf
+    x[5] = -inf
+    x[5, 65999] = -3.0
+    x[6] = torch.finfo(dtype).min
+    x[6, [2, 40000]] = 1.0
+    x[7] = torch.finfo(dtype).min
+    x[8] = 0.0
+    x[9] = torch.randint(0, 3, (vocab,), generator=g).to(dtype)
+    x[10] *= 1e4
+    x[11:20] = torch.randint(0, 40, (9, vocab), generator=g).to(dtype)
+    t[20], t[21], t[22], t[23] = 0.0, -1.0, 1e-30, 1e30
+    u[24], u[25], u[26] = 0.0, 2.0 ** -24, 1 - 2.0 ** -24
+    k, p, m = filters(n, vocab, g, vocab)
+    for kk, pp, mm in ((k, p, m), (None, p, None), (k, None, None), (None, None, None), (torch.full((n,), 7, dtype=torch.int32), None, None),
+                       (None, torch.full((n,), 0.5), torch.full((n,), 0.3))):
+        got, want = call(x, u, t, kk, pp, mm), expect(x, u, t, kk, pp, mm)
+        assert torch.equal(got, want), (torch.nonzero(got != want), got[got != want], want[got != want])
+
+
+def test_many_long_rows_strided_captured_and_beside_each_other():
+    """Unaligned rows of a wider tensor; the same tokens as row by row; two captured calls replayed on two streams."""
+    from llm_from_scratch_b200 import ops
+    for dtype in DTYPES:
+        wide, u, t, g = [v.cuda() if torch.is_tensor(v) else v for v in rows(140, 32010, dtype, 2)]
+        k, p, m = (v.cuda() for v in filters(140, 32000, g, 500))
+        for offset in (0, 1, 6):
+            part = wide[:, offset:offset + 32003]
+            got = ops.sample_filtered(part, u, t, k, p, m)
+            alone = torch.cat([ops.sample_filtered(part[i:i + 1], u[i:i + 1], t[i:i + 1], k[i:i + 1], p[i:i + 1], m[i:i + 1]) for i in range(140)])
+            assert torch.equal(got, alone)
+        graphs = []
+        for args in ((k, p, m), (None, p, None)):
+            torch.cuda.synchronize()
+            graph = torch.cuda.CUDAGraph()
+            want = ops.sample_filtered(wide, u, t, *args)
+            with torch.cuda.graph(graph):
+                out = ops.sample_filtered(wide, u, t, *args)
+            graphs.append((graph, out, want, torch.cuda.Stream()))
+        torch.cuda.synchronize()
+        for _ in range(4):
+            for graph, out, _, stream in graphs:
+                with torch.cuda.stream(stream):
+                    out.fill_(-1)
+                    graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(out, want) for _, out, want, _ in graphs)

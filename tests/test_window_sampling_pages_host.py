@@ -113,9 +113,12 @@ def test_argument_errors_of_the_library():
     dec = lambda **c: lib.b200_window_decode(*{**dict(q=x, k=x, v=x, out=x, bt=x, stride=2, width=2, lens=x, batch=1, Hq=4, Hkv=2, D=64, Dv=64, bs=16, nb=3,
                                                       scale=1.0, window=8, first=0, dtype=0, status=None, stream=None), **c}.values())
     assert dec(Hkv=3) == dec(window=-2) == dec(lens=None) == dec(bt=None) == -1 and dec(dtype=2) == -3 and dec(batch=0) == 0
-    smp = lambda **c: lib.b200_sample_filtered(*{**dict(logits=x, stride=9, rows=1, vocab=9, u=x, t=x, k=None, p=None, m=None, out=x, dtype=0, stream=None), **c}.values())
+    smp = lambda **c: lib.b200_sample_filtered(*{**dict(logits=x, stride=9, rows=1, vocab=9, u=x, t=x, k=None, p=None, m=None, out=x, ws=None, nbytes=0, dtype=0, stream=None), **c}.values())
     assert smp(vocab=0) == smp(stride=8) == smp(u=None) == smp(t=None) == smp(out=None) == -1
     assert smp(dtype=3) == -3 and smp(rows=0) == 0 and smp(vocab=(1 << 24) + 1, stride=1 << 25) == smp(rows=1 << 31) == -8
+    need = lib.b200_sample_filtered_workspace_bytes(300, 131072)
+    assert need > 0 and lib.b200_sample_filtered_workspace_bytes(1, 100) == lib.b200_sample_filtered_workspace_bytes(0, 131072) == 0
+    assert smp(rows=300, vocab=131072, stride=131072) == smp(rows=300, vocab=131072, stride=131072, ws=x, nbytes=need - 1) == -5
     cpy = lambda **c: lib.b200_copy_pages(*{**dict(pools=x, sizes=x, largest=64, n=1, pages=5, source=x, target=x, pairs=2, ws=None, nbytes=0, status=None, stream=None), **c}.values())
     assert cpy(pairs=-1) == cpy(source=None) == cpy(pools=None) == -1 and cpy(pairs=0) == cpy(n=0) == 0
     assert lib.b200_copy_pages_workspace_bytes(1024) == 0 and lib.b200_copy_pages_workspace_bytes(1025) == 4100
