@@ -28,9 +28,9 @@ struct alignas(16) RowState {
   int bin_k, left_k, bin_hi;
   int list_size, skip;                                    // skip: the row is in the list of the others
   // what the pass over the weights needs.  With y the distance from the maximum in bins: the bracket holds y_lo < y <= y_hi, the k-th token's bin
-  // y_k < y <= y_k1; beyond y_far weights do not count, and up to y_near a token may lie in front of the bracket or in a bin of the list.
-  float top, step, y_lo, y_hi, y_k, y_k1, y_far, y_near;
-  int all_weights;                                        // beyond y_near too
+  // y_k < y <= y_k1, and up to y_near a token may lie in front of the bracket or in a bin of the list.
+  float top, step, deep, y_lo, y_hi, y_k, y_k1, y_near;   // deep: logits below it weigh e^-64, which rounds to 0
+  int nucleus, at_k;
   double factor, floor_w;
 };
 
@@ -128,7 +128,8 @@ __device__ __forceinline__ RowParams row_params(const Wide& w, int row) {
   if (r.k >= a.vocab || r.k < 0) r.k = 0;
   const float floor_w = a.min_p ? a.min_p[row] : 0.f;
   r.floor_w = (floor_w > 1.f ? 1.0 : floor_w > 0.f ? static_cast<double>(floor_w) : 0.0) * static_cast<double>(1ull << a.bits);
-  r.taken = r.temperature > 0.f && fabsf(r.top) < INFINITY && r.u > 0.f;
+  // (the pass over the weights cuts distances at 64 T in 32 bits, which needs a T that is not lost beside the maximum)
+  r.taken = r.temperature > 0.f && fabsf(r.top) < INFINITY && r.u > 0.f && fabsf(r.top) < 1e6f * r.temperature;
   r.filtered = r.k > 0 || r.p < 1.f;
   r.factor = 64.0 * 1.4426950408889634 / r.temperature;
   r.reach = 660.f * r.temperature;
@@ -151,19 +152,19 @@ __global__ void __launch_bounds__(kThreads) wide_count_kernel(const Wide w) {
 #pragma unroll 4
   for (int i = blockIdx.x * w.count_tokens + tid * 4; i < end; i += kThreads * 4) {
     float v[4];
-    load4(x, i, V, wide, v);
+    load4_raw(x, i, V, wide, v);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const int b = min_of(__float2int_ru((r.top - v[j]) * r.step), kBins - 1);
-      if (b < last && i + j < V) atomicAdd(&hist[b >> 1], b & 1 ? 0x10000u : 1u);
+      const int b = __float2int_ru(fminf((r.top - v[j]) * r.step, kBins - 1.f));       // NaN goes to the last bin, as do places behind the row
+      if (b < last) atomicAdd(&hist[b & (kBins / 2 - 1)], b >= kBins / 2 ? 0x10000u : 1u);
     }
   }
   __syncthreads();
   uint32_t* out = w.hist + static_cast<int64_t>(row) * kBins;
   for (int i = tid; i < kBins / 2; i += kThreads) {
     const uint32_t y = hist[i];
-    if (y & 0xffff) atomicAdd(out + 2 * i, y & 0xffff);
-    if (y >> 16) atomicAdd(out + 2 * i + 1, y >> 16);
+    if (y & 0xffff) atomicAdd(out + i, y & 0xffff);
+    if (y >> 16) atomicAdd(out + kBins / 2 + i, y >> 16);
   }
 }
 
@@ -275,9 +276,9 @@ __global__ void __launch_bounds__(kRowThreads) wide_bracket_kernel(const Wide w)
       s.y_k1 = !at_k ? -1.f : bin_k < kBins - 1 ? bin_k : INFINITY;
       s.y_lo = nucleus ? bin_lo - 1.f : s.y_k;
       s.y_hi = nucleus ? hi : -1.f;
-      s.y_far = at_k ? fminf(s.y_k1, 660.f * kPerUnit) : 660.f * kPerUnit;
+      s.deep = r.top - 64.f * r.temperature;
       s.y_near = fmaxf(fmaxf(s.y_lo, s.y_hi), s.y_k1);
-      s.all_weights = nucleus;
+      s.nucleus = nucleus, s.at_k = at_k;
     }
   }
 }
@@ -290,8 +291,8 @@ __global__ void __launch_bounds__(kThreads) wide_sum_kernel(const Wide w) {
   if (s.skip) return;
   if (tid < 64) table[tid] = kTable[tid];
   __syncthreads();
-  const float top = s.top, step = s.step, y_lo = s.y_lo, y_hi = s.y_hi, y_k = s.y_k, y_k1 = s.y_k1, y_far = s.y_far, y_near = s.y_near;
-  const bool all_weights = s.all_weights;
+  const float top = s.top, step = s.step, deep = s.deep, y_lo = s.y_lo, y_hi = s.y_hi, y_k = s.y_k, y_k1 = s.y_k1, y_near = s.y_near;
+  const bool nucleus = s.nucleus, at_k = s.at_k;
   const double max = top, factor = s.factor, least = s.floor_w;
   const int S = w.a.bits;
   const T* x = static_cast<const T*>(w.a.logits) + row * w.a.row_stride;
@@ -307,28 +308,41 @@ __global__ void __launch_bounds__(kThreads) wide_sum_kernel(const Wide w) {
       float v[4], y[4];
       load4_raw(x, base + (c * 32 + lane) * 4, V, wide, v);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) y[j] = (top - v[j]) * step;          // NaN stays: no comparison holds for it
+      for (int j = 0; j < 4; ++j) {
+        y[j] = (top - v[j]) * step;                       // NaN stays: no comparison holds for it
+        v[j] = fmaxf(v[j], deep);
+      }
       const bool near = fminf(fminf(y[0], y[1]), fminf(y[2], y[3])) <= y_near;
-      if (!near && !all_weights) continue;
+      if (!near && !nucleus) continue;
       double g[4];
       unsigned long long m[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) g[j] = weight_unless(v[j], !(y[j] <= y_far), max, factor, S, table);
+      for (int j = 0; j < 4; ++j) g[j] = weight_within(v[j], max, factor, S, table), m[j] = rounded(g[j]);
+      if (at_k) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) m[j] = rounded(g[j]);
+        for (int j = 0; j < 4; ++j) m[j] = y[j] <= y_k1 ? m[j] : 0;
+      }
       all += (m[0] + m[1]) + (m[2] + m[3]);
-      if (near) {
+      if (!near) continue;
+      if (!at_k) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const bool before = y[j] <= y_lo, in = !before && (y[j] <= y_hi || (y[j] > y_k && y[j] <= y_k1));
+          const bool before = y[j] <= y_lo;
           if (before) front += m[j];
-          noted |= static_cast<uint32_t>(in) << (c * 4 + j);
+          if (!before && y[j] <= y_hi) noted |= 1u << (c * 4 + j);
         }
-        if (least > 0.0) {
+      } else {
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            if (y[j] <= y_lo && g[j] >= least) kept += m[j];
+        for (int j = 0; j < 4; ++j) {
+          const bool before = y[j] <= y_lo;
+          if (before) front += m[j];
+          if (!before && (y[j] <= y_hi || (y[j] > y_k && y[j] <= y_k1))) noted |= 1u << (c * 4 + j);
         }
+      }
+      if (least > 0.0) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (y[j] <= y_lo && g[j] >= least) kept += m[j];
       }
     }
     if (__any_sync(0xffffffffu, noted)) {                 // one addition to the list's size per warp
@@ -341,7 +355,7 @@ __global__ void __launch_bounds__(kThreads) wide_sum_kernel(const Wide w) {
         const float v = i < V ? to_float<T>(x[i]) : -INFINITY;         // no NaN is in the list
         if (at < kList) {
           w.list_key[static_cast<int64_t>(row) * kList + at] = composite(v, i);
-          w.list_mass[static_cast<int64_t>(row) * kList + at] = rounded(weight_unless(v, !((top - v) * step <= y_far), max, factor, S, table));
+          w.list_mass[static_cast<int64_t>(row) * kList + at] = rounded(weight_within(fmaxf(v, deep), max, factor, S, table));
         }
       }
     }
@@ -353,8 +367,11 @@ __global__ void __launch_bounds__(kThreads) wide_sum_kernel(const Wide w) {
   }
 }
 
+constexpr int kBuckets = 4096, kOwnBuckets = kBuckets / kRowThreads;
+
 struct DrawShared {
-  unsigned long long key[kList], mass[kList], chunk[kMaxChunks], scan[kRowThreads / 32], total[2];
+  unsigned long long key[kList], mass[kList], chunk[kMaxChunks], scan[kRowThreads / 32];
+  int bucket[kBuckets];                                   // tokens, then the place of the first one, of a step of the list's bins
   double table[64];
   int place, chunk_at;
   unsigned long long left;
@@ -380,14 +397,57 @@ __global__ void __launch_bounds__(kRowThreads) wide_draw_kernel(const Wide w) {
   auto bin_of = [&](unsigned long long key) {
     return min_of(__float2int_ru((r.top - key_value(static_cast<uint32_t>(key >> 32))) * r.step), kBins - 1);
   };
-  // ---- the list in order
+  // ---- the list in order: tokens are counted and placed by fine steps of the bracket and of the k-th token's bin (0 .. 2,047 and behind them),
+  // then by the number of those before them in their step
   unsigned long long listed_all = 0;
-  for (int i = tid; i < size; i += kRowThreads) {
-    sh.key[i] = w.list_key[static_cast<int64_t>(row) * kList + i];
-    sh.mass[i] = w.list_mass[static_cast<int64_t>(row) * kList + i];
-    listed_all += sh.mass[i];
+  {
+    unsigned long long key[kOwnList], mass[kOwnList];
+    int bucket[kOwnList], count[kOwnBuckets], own = 0, all;
+    const float near = 2047.f / (s.y_hi - s.y_lo), far = 2047.f / (s.y_k1 - s.y_k);
+    for (int i = tid; i < kBuckets; i += kRowThreads) sh.bucket[i] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < kOwnList; ++j) {
+      const int i = tid + j * kRowThreads;
+      if (i >= size) break;
+      key[j] = w.list_key[static_cast<int64_t>(row) * kList + i];
+      mass[j] = w.list_mass[static_cast<int64_t>(row) * kList + i];
+      listed_all += mass[j];
+      const float y = (r.top - key_value(static_cast<uint32_t>(key[j] >> 32))) * r.step;
+      bucket[j] = y <= s.y_hi ? __float2int_ru(fminf(fmaxf((y - s.y_lo) * near, 0.f), 2047.f))
+                              : 2048 + __float2int_ru(fmaxf(fminf((y - s.y_k) * far, 2047.f), 0.f));        // NaN, of infinities, to the end
+      atomicAdd(&sh.bucket[bucket[j]], 1);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int c = 0; c < kOwnBuckets; ++c) count[c] = sh.bucket[tid * kOwnBuckets + c], own += count[c];
+    int first = block_upto(own, reinterpret_cast<int*>(sh.scan), all) - own;
+#pragma unroll
+    for (int c = 0; c < kOwnBuckets; ++c) sh.bucket[tid * kOwnBuckets + c] = first, first += count[c];
+    __syncthreads();
+    int slot[kOwnList];
+#pragma unroll
+    for (int j = 0; j < kOwnList; ++j) {
+      if (tid + j * kRowThreads >= size) break;
+      slot[j] = atomicAdd(&sh.bucket[bucket[j]], 1);      // afterwards the place behind the bucket
+      sh.key[slot[j]] = key[j];
+    }
+    __syncthreads();
+    int place[kOwnList];
+#pragma unroll
+    for (int j = 0; j < kOwnList; ++j) {
+      if (tid + j * kRowThreads >= size) break;
+      const int begin = bucket[j] > 0 ? sh.bucket[bucket[j] - 1] : 0, end = sh.bucket[bucket[j]];
+      place[j] = begin;
+      for (int i = begin; i < end; ++i) place[j] += sh.key[i] > key[j];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < kOwnList; ++j) {
+      if (tid + j * kRowThreads >= size) break;
+      sh.key[place[j]] = key[j], sh.mass[place[j]] = mass[j];
+    }
   }
-  sort_by_key<kRowThreads>(sh.key, sh.mass, size);
   // ---- sums in front of the list and behind it
   unsigned long long front = 0, rest = 0, ignored;
   const unsigned long long* sums = w.sums + static_cast<int64_t>(row) * w.chunks * 3;

@@ -53,17 +53,20 @@ __device__ const double kTable[64] = {
     1.9152065613971474, 1.9360617934922943, 1.9571441241754002, 1.978456026387951};
 
 // The weight in units of 2^-S: 2^(n / 64) 2^(r / 64) with |r| <= 1/2, the second factor by its series up to r^4 (error 4e-14).
-__device__ __forceinline__ double weight_unless(float x, bool far, double max, double factor, int S, const double* table) {
+// For logits no further from the maximum than 600 T.
+__device__ __forceinline__ double weight_within(float x, double max, double factor, int S, const double* table) {
   const double y = (static_cast<double>(x) - max) * factor;
   const double t = y + kMagic, r = y - (t - kMagic);
   const int n = __double2loint(t);
   constexpr double b = 0.010830424696249145;             // ln 2 / 64
   const double q = fma(r, fma(r, fma(r, fma(r, b * b * b * b / 24, b * b * b / 6), b * b / 2), b), 1.0);
   const double v = table[n & 63] * q;
-  return far ? 0.0 : __hiloint2double(__double2hiint(v) + (((n >> 6) + S) << 20), __double2loint(v));
+  return __hiloint2double(__double2hiint(v) + (((n >> 6) + S) << 20), __double2loint(v));
 }
+// For any: 0 beyond `reach`.
 __device__ __forceinline__ double weight_of(float x, float top, double max, double factor, float reach, int S, const double* table) {
-  return weight_unless(x, top - x > reach, max, factor, S, table);
+  const double w = weight_within(x, max, factor, S, table);
+  return top - x > reach ? 0.0 : w;
 }
 
 // A weight as a whole number, below 2^51; 0 for weights below e^-32 where the unit is 2^-45.
