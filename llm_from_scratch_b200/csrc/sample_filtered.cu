@@ -8,7 +8,8 @@
 // Rows with T <= 0 and rows without any weight (no logit above -inf) take the first of the highest logits.  NaN counts as -inf.
 //
 // Weights are computed in 64 bits and held as whole numbers of 2^-S, S as large as their sum allows (45 bits at 131,072
-// tokens, no more in the clustered kernel): sums of whole numbers do not depend on their order, so the borders fall at the same token whatever the launch looks like.
+// tokens, no more in the clustered kernel): sums of whole numbers do not depend on their order, so the borders fall at the same token whatever
+// the launch looks like.
 //
 // A cluster of CTAs shares a row, whose logits stay in shared memory: a thread owns a run of neighbouring tokens.  Borders by value (top-k with
 // ones as masses, top-p with the weights) are found with a histogram over the distance from the maximum, in steps of T / 128, and, if the
@@ -970,9 +971,13 @@ __global__ void __launch_bounds__(kThreads) sample_filtered_kernel(const SampleA
 
 bool fits_cluster(int vocab) { return row_smem(vocab, 8) <= 226 * 1024 && row_shape(vocab, 8).slice < 65536; }
 
-// Whether passes of separate launches are faster than clusters.
+// Whether passes of separate launches are faster than clusters.  Measured (us, clusters / passes, top-p, fp32 unless told otherwise): 16 rows of
+// 131,072 41 / 34, 32 73 / 40, 64 104 / 54, 256 341 / 142, 256 of bf16 490 / 175; 64 rows of 65,536 46 / 40; 192 rows of 32,000 51 / 50, 256 with
+// all filters 61 / 57, 64 24 / 36; 512 rows of 16,384 65 / 72, of 8,192 45 / 60; without filters 512 rows of 32,000 47 / 65, 256 of 131,072
+// 106 / 99.  Below 65,536 tokens the two are even at best, and the passes take the host 14 us longer to launch and need the workspace.  They lose
+// at bf16 and few rows with a small k: 32 rows of 131,072 31 / 52.
 bool wide_is_faster(int64_t rows, int vocab) {
-  return fits_cluster(vocab) && sample_wide_takes(rows, vocab) && vocab >= 16384 && rows * vocab >= (int64_t(1) << 22);
+  return fits_cluster(vocab) && sample_wide_takes(rows, vocab) && vocab >= 65536 && rows * vocab >= (int64_t(1) << 22);
 }
 
 }  // namespace

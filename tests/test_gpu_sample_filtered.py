@@ -168,7 +168,7 @@ def test_captured_and_on_two_streams():
 
 # ------------------------------------------------------------------------------------------------ many long rows: passes of separate launches
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("n,vocab,most,spread", [(130, 33000, 1000, (0.5, 8.0)), (260, 16384, 16384, (0.5, 8.0)), (33, 131072, 50000, (0.05, 3.0)),
+@pytest.mark.parametrize("n,vocab,most,spread", [(65, 66000, 1000, (0.5, 8.0)), (64, 65536, 65536, (0.5, 8.0)), (33, 131072, 50000, (0.05, 3.0)),
                                                  (45, 100001, 60, (1.0, 12.0))])
 def test_many_long_rows(n, vocab, most, spread, dtype):
     from llm_from_scratch_b200._lib import lib
@@ -215,12 +215,12 @@ def test_many_long_rows_strided_captured_and_beside_each_other():
     """Unaligned rows of a wider tensor; the same tokens as row by row; two captured calls replayed on two streams."""
     from llm_from_scratch_b200 import ops
     for dtype in DTYPES:
-        wide, u, t, g = [v.cuda() if torch.is_tensor(v) else v for v in rows(140, 32010, dtype, 2)]
-        k, p, m = (v.cuda() for v in filters(140, 32000, g, 500))
+        wide, u, t, g = [v.cuda() if torch.is_tensor(v) else v for v in rows(66, 66010, dtype, 2)]
+        k, p, m = (v.cuda() for v in filters(66, 66000, g, 500))
         for offset in (0, 1, 6):
-            part = wide[:, offset:offset + 32003]
+            part = wide[:, offset:offset + 66003]
             got = ops.sample_filtered(part, u, t, k, p, m)
-            alone = torch.cat([ops.sample_filtered(part[i:i + 1], u[i:i + 1], t[i:i + 1], k[i:i + 1], p[i:i + 1], m[i:i + 1]) for i in range(140)])
+            alone = torch.cat([ops.sample_filtered(part[i:i + 1], u[i:i + 1], t[i:i + 1], k[i:i + 1], p[i:i + 1], m[i:i + 1]) for i in range(66)])
             assert torch.equal(got, alone)
         graphs = []
         for args in ((k, p, m), (None, p, None)):
@@ -238,3 +238,17 @@ def test_many_long_rows_strided_captured_and_beside_each_other():
                     graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(out, want) for _, out, want, _ in graphs)
+
+
+# ------------------------------------------------------------------------------------------------ vocabularies beyond a cluster's shared memory
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_vocabularies_beyond_a_cluster(dtype):
+    n, vocab = 6, 500_001
+    x, u, t, g = rows(n, vocab, dtype, 11)
+    x[1] = -math.inf
+    x[2, 17] = math.inf
+    x[3, ::3] = math.nan
+    t[4] = 0.0
+    k, p, m = filters(n, vocab, g, 5000)
+    for kk, pp, mm in ((k, p, m), (k, None, None), (None, p, None), (None, None, m), (None, None, None)):
+        assert torch.equal(call(x, u, t, kk, pp, mm), expect(x, u, t, kk, pp, mm))
