@@ -843,7 +843,7 @@ int b200_sample_filtered(const void* logits, int64_t row_stride, int64_t num_row
  * of which largest_page is the largest.
  * Page target[j] of every pool becomes page source[j]; pairs with a negative id are left out, ids outside the pool reported.  A pair
  * whose target is also a source of the call or the target of an earlier pair is not carried out and reported (B200_ERR_ARG). */
-size_t b200_copy_pages_workspace_bytes(int32_t num_pairs);
+size_t b200_copy_pages_workspace_bytes(int32_t num_pairs, int64_t num_pages);
 int b200_copy_pages(const int64_t* pools, const int64_t* page_bytes, int64_t largest_page, int32_t num_pools, int64_t num_pages,
                     const int32_t* source, const int32_t* target, int32_t num_pairs, void* workspace, size_t workspace_bytes, int32_t* status,
                     void* stream);

@@ -134,7 +134,7 @@ SIGNATURES = {
                                   _vp, _vp]),
     "b200_sample_filtered_workspace_bytes": (_sz, [_i64, _i32]),
     "b200_sample_filtered": (_i32, [_vp, _i64, _i64, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _i32, _vp]),
-    "b200_copy_pages_workspace_bytes": (_sz, [_i32]),
+    "b200_copy_pages_workspace_bytes": (_sz, [_i32, _i64]),
     "b200_copy_pages": (_i32, [_vp, _vp, _i64, _i32, _i64, _vp, _vp, _i32, _vp, _sz, _vp, _vp]),
     "b200_compact_pages": (_i32, [_vp, _vp, _i64, _i32, _i64, _vp, _i64, _i64, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
     "b200_selftest_bounded_wait": (_i32, [_i32, _vp, _vp, _vp]),

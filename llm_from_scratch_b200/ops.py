@@ -1714,6 +1714,8 @@ def sample_filtered(logits: torch.Tensor, uniforms: torch.Tensor, temperatures: 
     if logits.dim() != 2 or logits.shape[1] == 0:
         raise ValueError("logits must be [B, V]")
     B, V = logits.shape
+    if V > 1 << 24:
+        raise ValueError("at most 2^24 tokens to choose from")
     if V > 1 and logits.stride(1) != 1:
         raise ValueError("logits rows must be contiguous")
     if B > 1 and logits.stride(0) < V:
@@ -1777,7 +1779,9 @@ def copy_pages(pools: PagePools, source: torch.Tensor, target: torch.Tensor) -> 
     if source.numel() != target.numel():
         raise ValueError("source and target must have the same length")
     n = source.numel()
-    nbytes = lib.b200_copy_pages_workspace_bytes(n)
+    if n > 0x7FFFFFFF:
+        raise ValueError("at most 2^31 - 1 pairs")
+    nbytes = lib.b200_copy_pages_workspace_bytes(n, pools.num_pages)
     scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
     check(lib.b200_copy_pages(*pools._args, source.data_ptr(), target.data_ptr(), n, _ptr(scratch), nbytes,
                               status_word(dev).data_ptr(), _stream()), "copy_pages")

@@ -121,8 +121,8 @@ def test_argument_errors_of_the_library():
     assert smp(rows=300, vocab=131072, stride=131072) == smp(rows=300, vocab=131072, stride=131072, ws=x, nbytes=need - 1) == -5
     cpy = lambda **c: lib.b200_copy_pages(*{**dict(pools=x, sizes=x, largest=64, n=1, pages=5, source=x, target=x, pairs=2, ws=None, nbytes=0, status=None, stream=None), **c}.values())
     assert cpy(pairs=-1) == cpy(source=None) == cpy(pools=None) == -1 and cpy(pairs=0) == cpy(n=0) == 0
-    assert lib.b200_copy_pages_workspace_bytes(1024) == 0 and lib.b200_copy_pages_workspace_bytes(1025) == 4100
-    assert cpy(pairs=1025) == cpy(pairs=1025, ws=x, nbytes=4099) == -5
+    assert lib.b200_copy_pages_workspace_bytes(1024, 700) == 0 and lib.b200_copy_pages_workspace_bytes(1025, 700) == 2800
+    assert cpy(pairs=1025) == cpy(pairs=1025, ws=x, nbytes=19) == -5 and cpy(pairs=0x7fffffff) == cpy(pages=1 << 31) == -8
     cmp_ = lambda **c: lib.b200_compact_pages(*{**dict(pools=x, sizes=x, largest=64, n=1, pages=5, bt=x, stride=2, rows=3, width=2, out=x, map=x, source=x, target=x, counts=x,
                                                        status=None, stream=None), **c}.values())
     assert cmp_(stride=1) == cmp_(bt=None) == cmp_(map=None) == cmp_(counts=None) == cmp_(rows=-1) == -1 and cmp_(pages=1 << 31) == -8
