@@ -310,7 +310,7 @@ int window_decode_launch(const WindowArgs& a, cudaStream_t s) {
   int64_t keys = static_cast<int64_t>(a.bt_width) * a.bs;               // that a sequence may see
   if (keys > static_cast<int64_t>(a.window) + a.first) keys = static_cast<int64_t>(a.window) + a.first;
   int ranks = 1;
-  while (ranks < 8 && static_cast<int64_t>(ranks) * kWarps * kTok < keys && units * ranks * 2 <= wave * (keys / ranks > 1024 ? 2 : 1)) ranks *= 2;
+  while (ranks < 8 && static_cast<int64_t>(ranks) * kWarps * kTok < keys && units * ranks * 2 <= wave) ranks *= 2;
   if (G > 8) return a.D == 128 ? launch<128, 2>(p, ranks, s) : launch<64, 2>(p, ranks, s);
   return a.D == 128 ? launch<128, 1>(p, ranks, s) : launch<64, 1>(p, ranks, s);
 }

@@ -43,7 +43,7 @@ struct Lay {
   static constexpr int OFF_KV = NP * Q_BYTES, OFF_BAR = OFF_KV + NST * STAGE;
   // as in prefill_umma2.cu
   static constexpr int Q_FULL = 0, K_FULL = 1, V_FULL = 1 + NST, QK_DONE = 1 + 2 * NST, PV_DONE = 1 + 4 * NST, P_READY = 1 + 6 * NST,
-                       TURN = P_READY + 4, NUM_BARS = TURN + 8;
+                       TURN = P_READY + 4, LEFT = TURN + 8, NUM_BARS = LEFT + NP;
   static constexpr int SMEM = OFF_BAR + NUM_BARS * 8 + 32 + 1024;
   static constexpr int TCOLS = NP * (128 + D) > 256 ? 512 : 256;
 };
@@ -146,6 +146,7 @@ window_prefill_kernel(const PromptArgs p, const __grid_constant__ CUtensorMap tm
     }
     for (int i = 0; i < 4; ++i) umma::mbar_init(bar(L::P_READY + i), 128);
     for (int i = 0; i < 8; ++i) umma::mbar_init(bar(L::TURN + i), 32);
+    for (int x = 0; x < NP; ++x) umma::mbar_init(bar(L::LEFT + x), 1);
     *s_abort = 0;
     umma::mbar_init_fence();
   }
@@ -186,6 +187,7 @@ window_prefill_kernel(const PromptArgs p, const __grid_constant__ CUtensorMap tm
     break;                                                           \
   }
 
+  int issued = 0;                            // key tiles that this producer has asked for
   if (warp < 2) {
     // =============================== TMA producers ===============================
     const bool is_k = warp == 0;
@@ -232,6 +234,7 @@ window_prefill_kernel(const PromptArgs p, const __grid_constant__ CUtensorMap tm
       if (mine)
         umma::tma_load_3d(sb + L::OFF_KV + st * L::STAGE + (is_k ? 0 : L::K_BYTES) + slab * K_SLAB + part * p.box * 128, is_k ? &tm_k : &tm_v,
                           slab * 64, kvh, static_cast<int>(row), bar(full0 + st));
+      issued = j + 1;
     }
   } else if (warp < 4) {
     // =============================== MMA issuers ===============================
@@ -459,6 +462,18 @@ window_prefill_kernel(const PromptArgs p, const __grid_constant__ CUtensorMap tm
 #undef WAIT_OR_ABORT
   umma::fence_before_sync();
   __syncthreads();
+  if (*s_abort) {                            // uniform: nobody sets it any more.  Copies and products under way end before the CTA does
+    volatile int never = 0;
+    if (warp < 2 && lane == 0) {
+      for (int t = max(issued - NST, 0); t < issued; ++t)
+        umma::mbar_wait(bar((warp == 0 ? L::K_FULL : L::V_FULL) + t % NST), (t / NST) & 1, &never);
+      if (warp == 0) umma::mbar_wait(bar(L::Q_FULL), 0, &never);
+    } else if (warp < 2 + NP && lane == 0) {
+      umma::commit(bar(L::LEFT + warp - 2));
+      umma::mbar_wait(bar(L::LEFT + warp - 2), 0, &never);
+    }
+    __syncthreads();
+  }
   if (warp == 2) umma::tmem_dealloc(tmem, L::TCOLS);
   if (s_again && !*s_abort) {
     const int all = (toks[0] + toks[1]) * p.G;
