@@ -14,7 +14,7 @@
 // A cluster of CTAs shares a row, whose logits stay in shared memory: a thread owns a run of neighbouring tokens.  Borders by value (top-k with
 // ones as masses, top-p with the weights) are found with a histogram over the distance from the maximum, in steps of T / 128, and, if the
 // border's bin holds more than a few tokens, over ever finer ranges of the logits' bits; what is left is sorted.  The border of the draw is
-// found by sums over the threads' runs.  Histograms hold a weight in three parts of 16 bits or more, each a 32-bit counter: shared memory adds
+// found by sums over the threads' runs.  Many long rows go through sample_wide.cu.  Histograms hold a weight in three parts of 16 bits or more, each a 32-bit counter: shared memory adds
 // 32 bits at a time.
 //
 // Bound by the reads for large rows in principle; in fact by the weights (ten 64-bit operations each) and the histogram's additions.
@@ -612,10 +612,12 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, const int row, u
     int bin_lo = kBins, bin_hi = kBins - 1;              // bins among which the nucleus ends
     int listed = count_k;                                // tokens of the list
     if (nucleus) {
+      // 3.5 standard deviations: a row whose border lies outside, or whose bracket has more tokens than the list takes, finds it by the histograms
+      // of weights.  Mean of 20 calls of 64 rows of 32,000, all filters: 28.6 us; with four 29.1, with five and 1e-4 31.2
       auto off = [&](float m, float e) {
         float root;
         asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(root) : "f"(e));
-        return sizeof(T) == 2 ? e + 1e-5f * m : 5.f * root + 1e-4f * m;
+        return sizeof(T) == 2 ? e + 1e-5f * m : 3.5f * root + 1e-5f * m;
       };
       const float goal = p * mass_all, wide = p * off(mass_all, spread_all);
       if (busy && mass_up + off(mass_up, spread_up) + wide >= goal && !(mass_up - mass - off(mass_up - mass, spread_up - spread) - wide >= goal)) {
@@ -971,11 +973,11 @@ __global__ void __launch_bounds__(kThreads) sample_filtered_kernel(const SampleA
 
 bool fits_cluster(int vocab) { return row_smem(vocab, 8) <= 226 * 1024 && row_shape(vocab, 8).slice < 65536; }
 
-// Whether passes of separate launches are faster than clusters.  Measured (us, clusters / passes, top-p, fp32 unless told otherwise): 16 rows of
-// 131,072 41 / 34, 32 73 / 40, 64 104 / 54, 256 341 / 142, 256 of bf16 490 / 175; 64 rows of 65,536 46 / 40; 192 rows of 32,000 51 / 50, 256 with
-// all filters 61 / 57, 64 24 / 36; 512 rows of 16,384 65 / 72, of 8,192 45 / 60; without filters 512 rows of 32,000 47 / 65, 256 of 131,072
-// 106 / 99.  Below 65,536 tokens the two are even at best, and the passes take the host 14 us longer to launch and need the workspace.  They lose
-// at bf16 and few rows with a small k: 32 rows of 131,072 31 / 52.
+// Whether passes of separate launches are faster than clusters.  Measured (us, clusters / passes, top-p and fp32 unless told otherwise, means over
+// eight draws): 16 rows of 131,072 42 / 35, 32 49 / 39, 64 71 / 52, 256 341 / 159, 256 of bf16 480 / 169; 16 rows of 262,144 72 / 40; 64 rows of
+// 65,536 42 / 39; with all filters 64 rows of 32,000 27 / 35, 256 55 / 57, top-p alone 512 109 / 95, 256 of bf16 88 / 81; 512 rows of 16,384
+// 61 / 69, of 8,192 45 / 57; without filters 512 rows of 32,000 47 / 60, 256 of 131,072 106 / 99.  Below 65,536 tokens neither is much ahead,
+// and the passes take the host 14 us longer to launch and need a workspace.  They lose at bf16 with a small k: 64 rows of 131,072 60 / 72.
 bool wide_is_faster(int64_t rows, int vocab) {
   return fits_cluster(vocab) && sample_wide_takes(rows, vocab) && vocab >= 65536 && rows * vocab >= (int64_t(1) << 22);
 }

@@ -239,10 +239,12 @@ __global__ void __launch_bounds__(kRowThreads) wide_bracket_kernel(const Wide w)
       const float e = g * (1.f / kPerUnit) * (sizeof(T) == 2 ? 0.005f * n : 0.29f), f = sizeof(T) == 2 ? e : e * e * n;
       return b == 0 ? 0.f : f;
     };
+    // four standard deviations: a border outside costs its row the other form (75 us), as does a bracket of more tokens than the list takes.
+    // Mean of 20 calls of 256 rows of 131,072, p up to 0.99: 159 us; with five and 1e-4 182 (11 rows went, not 4)
     auto off = [&](float m, float e) {
       float root;
       asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(root) : "f"(e));
-      return sizeof(T) == 2 ? e + 1e-5f * m : 5.f * root + 1e-4f * m;
+      return sizeof(T) == 2 ? e + 1e-5f * m : 4.f * root + 1e-5f * m;
     };
     int counted = 0;
     float mass = 0.f, spread = 0.f;
