@@ -13,7 +13,9 @@
 // reduction of every score the latter took 457 us.
 //
 // WINDOW: a token sees the last `window` tokens of its context and its first ones (window_attention.cu).  The visible tokens are numbered
-// through, first tokens first, and what follows cuts and walks these numbers; a share with tokens of both parts is walked in two.
+// through, first tokens first, and what follows cuts and walks these numbers.  64 sequences of 64 .. 2,048 tokens with a window of 500 and 5 first
+// tokens, 16/4 x 64: 14.3 us, of them
+// 7 for the 45 MB of rows.
 #include <cooperative_groups.h>
 
 #include "sequences.cuh"
@@ -103,13 +105,17 @@ __global__ void __launch_bounds__(kThreads, 3) decode_f32_kernel(const DecodeF32
   const int shift = (a.bs & (a.bs - 1)) == 0 ? __ffs(a.bs) - 1 : -1;
   auto page_of = [&](int t) { return shift >= 0 ? t >> shift : t / a.bs; };
   float4* slots = ring + (warp * kStages * kUnroll * 4) * 32 + lane;
-  const int span = static_cast<int>(min(static_cast<int64_t>(kTable - 1) * a.bs, static_cast<int64_t>(len)));
-  auto walk = [&](const int from, const int to) {
-  for (int base = from; base < to; base += span) {
-    const int end = min(base + span, to), page0 = page_of(base), pages = page_of(end - 1) - page0 + 1;
+  const int span = static_cast<int>(min(static_cast<int64_t>(kTable - (WINDOW ? 4 : 1)) * a.bs, static_cast<int64_t>(len)));
+  for (int base = lo; base < hi; base += span) {
+    const int end = min(base + span, hi);
+    // WINDOW: a share with tokens of both parts has the pages of the first tokens in front of the window's
+    const bool both = WINDOW && base < front && end > front;
+    auto position = [&](int t) { return WINDOW && t >= front ? t + gap : t; };
+    const int page0 = page_of(position(base)), pages0 = both ? page_of(front - 1) - page0 + 1 : 0, page1 = both ? page_of(front + gap) : page0;
+    const int pages = pages0 + page_of(position(end - 1)) - page1 + 1;
     __syncthreads();
     for (int i = tid; i < pages; i += kThreads) {
-      int id = table[page0 + i];
+      int id = table[i < pages0 ? page0 + i : page1 + i - pages0];
       if (static_cast<uint64_t>(static_cast<int64_t>(id)) >= static_cast<uint64_t>(a.num_blocks)) {
         report(a.status, B200_ERR_BOUNDS);
         id = -1;
@@ -125,10 +131,11 @@ __global__ void __launch_bounds__(kThreads, 3) decode_f32_kernel(const DecodeF32
       valid <<= kUnroll;
 #pragma unroll
       for (int u = 0; u < kUnroll; ++u) {
-        const int t = first + i * TRIP + u * TW, page = page_of(min(t, end - 1)), id = s_table[page - page0];
+        const int t = first + i * TRIP + u * TW, at = position(min(t, end - 1)), page = page_of(at);
+        const int id = s_table[both && t < front ? page - page0 : page - page1 + pages0];
         const bool in = t < end && id >= 0;
         if (in) valid |= 1u << u;
-        const int64_t row = in ? ((static_cast<int64_t>(id) * a.bs + (t - page * a.bs)) * a.Hkv + kvh) * D + sub * 4 : 0;
+        const int64_t row = in ? ((static_cast<int64_t>(id) * a.bs + (at - page * a.bs)) * a.Hkv + kvh) * D + sub * 4 : 0;
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           cp_async16(smem_u32(dst + (u * 4 + c) * 32), a.kc + row + (in ? c * LP * 4 : 0), in ? 16 : 0);
@@ -240,9 +247,6 @@ __global__ void __launch_bounds__(kThreads, 3) decode_f32_kernel(const DecodeF32
     }
     cp_async_wait<0>();
   }
-  };
-  if (WINDOW && lo < front) walk(lo, min(hi, front));
-  walk(WINDOW ? max(lo, front) + gap : lo, hi + gap);
   // ---- lane groups of the warp, warps of the CTA, CTAs of the cluster ----
 #pragma unroll
   for (int g = 0; g < GC; ++g) {
@@ -342,14 +346,19 @@ int launch_dim(const DecodeF32Args& a, int batch, cudaStream_t s) {
   // round; the line is where the times lie, not a wave (one, two, four, eight CTAs per context, 64 .. 1,024 tokens: 64 sequences at 16/4 x
   // 64 19.5, 17.0, 19.2, 25.8 us, 32 at 32/8 x 128 34, 32, 38, 52; 128 .. 8,192 tokens, 64 at 16/4 x 64 129, 75, 64, 65).
   const int64_t pairs = static_cast<int64_t>(batch) * (a.Hq / GC), seen = static_cast<int64_t>(a.window) + a.first;
-  const int64_t table = (WINDOW ? a.bt_width : a.bt_stride) * a.bs, keys = WINDOW && seen < table ? seen : table;
+  const int64_t table = (WINDOW ? a.bt_width : a.bt_stride) * a.bs;
+  // A window shorter than the tables makes long contexts equal: at most three CTAs an SM then (one, two, four, eight per context, 64 sequences at
+  // 16/4 x 64: 64 .. 2,048 tokens, window 500, 14.3, 17.5, 20.8, 27.5 us; 2,048 .. 8,192, window 4,096, 84, 103, 91, 99; 16 of 64 .. 2,048
+  // 12.0, 8.7, 8.0, 8.2; 32 at 32/8 x 128, window 1,024, 42, 43, 48, 66).
+  const bool cut = WINDOW && seen < table;
+  const int64_t keys = cut ? seen : table;
   // The general kernel keeps contexts of up to eight tokens, where the merges are the call (one token at 16/4 x 64: 4.7 against 2.8 us), and
   // large batches of up to sixteen where no heads share the rows (256 x 16 at 16/16 x 32: 28 against 19).
   if (keys <= 8 || (keys <= 16 && GC == 1 && pairs >= 2048)) return B200_ERR_UNSUPPORTED;
   const int trip = kWarps * (32 / (D / 8)) * kUnroll;
   int ranks = 1;
   while (ranks < 8 && static_cast<int64_t>(ranks) * trip < keys &&
-         pairs * ranks * 2 <= (keys / ranks > 1024 ? 8 : 4) * static_cast<int64_t>(sms))
+         pairs * ranks * 2 <= (cut ? 3 : keys / ranks > 1024 ? 8 : 4) * static_cast<int64_t>(sms))
     ranks *= 2;
   if (GC == 4) return launch_heads<D, 4, WINDOW>(a, batch, ranks, s);
   if (GC == 2) return launch_heads<D, 2, WINDOW>(a, batch, ranks, s);

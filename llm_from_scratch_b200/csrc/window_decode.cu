@@ -5,8 +5,11 @@
 // cluster's distributed shared memory.  The window bounds the work of a sequence, and the host knows it, so no pass over the lengths is needed
 // and there is no scratch in global memory.  Products and softmax are those of decode_cluster.cu: the query heads are the N dimension
 // of mma.sync m16n8k16 (a decode step has too few rows for tcgen05, and the tensor pipe idles either way), S^T = K Q^T and O^T = V^T P^T,
-// scores and sums in fp32, weights rounded to bf16 for the second product.  Rows arrive by cp.async, swizzled, blocks ahead; a row that is not
-// visible is not read, zeros take its place.
+// scores and sums in fp32, weights rounded to bf16 for the second product (2^-8 of a weight, and the tensor cores take nothing wider beside
+// bf16 values).  Rows arrive by cp.async, swizzled, blocks ahead; a row that is not visible is not read, zeros take its place.
+//
+// Measured at 32/8 x 128: a sequence with a window of 1,024 and 4 first tokens 6.2 us, of which a launch is half and the rest a chain of dependent
+// reads (length, table, rows) and the two merges; 256 sequences with a window of 4,096, 2.08 GB of rows, 315 us, 6.6 TB/s.
 #include <cooperative_groups.h>
 
 #include "window_attention.cuh"
@@ -309,6 +312,9 @@ int window_decode_launch(const WindowArgs& a, cudaStream_t s) {
   const int64_t units = static_cast<int64_t>(a.num_seqs) * a.Hkv * p.chunks, wave = 2 * static_cast<int64_t>(sms);
   int64_t keys = static_cast<int64_t>(a.bt_width) * a.bs;               // that a sequence may see
   if (keys > static_cast<int64_t>(a.window) + a.first) keys = static_cast<int64_t>(a.window) + a.first;
+  // CTAs per (sequence, KV head): doubled up to two an SM, none with fewer than four blocks of its own (one, two, four, eight, 32/8 x 128: 1 sequence
+  // with 512 visible keys 9.3, 7.2, 6.0, 5.6 us, with 16,384 173, 89, 47, 26; 16 with 1,024 15.6, 15.4, 19.9, 29.1, with 16,384 175, 161,
+  // 161, 169; 64 with 512 28, 38, 51, 88, with 4,096 158, 163, 172, 201)
   int ranks = 1;
   while (ranks < 8 && static_cast<int64_t>(ranks) * kWarps * kTok < keys && units * ranks * 2 <= wave) ranks *= 2;
   if (G > 8) return a.D == 128 ? launch<128, 2>(p, ranks, s) : launch<64, 2>(p, ranks, s);
