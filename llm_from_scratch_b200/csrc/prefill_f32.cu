@@ -13,7 +13,8 @@
 // faster; in the general grid's order, one sequence after the other, the kernel took 80 us more.
 //
 // WINDOW (paged keys): a query sees the last `window` tokens and the first ones (window_attention.cu).  The walk goes over the tiles with
-// first tokens and then those from the start of the first row's window on; keys that no row sees are not read.
+// first tokens and then those from the start of the first row's window on; keys that no row sees are not read.  24 portions of 1 .. 1,000 tokens, 3,930 in all, behind
+// up to 8,000, 16/4 x 64, window 1,024: 605 us.
 #include "sequences.cuh"
 #include "window_attention.cuh"
 

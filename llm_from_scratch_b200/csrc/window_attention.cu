@@ -5,7 +5,9 @@
 //
 // General kernel: a warp per (query token, query head), every element type, head size and page size.  A lane owns the head-dim
 // elements lane, lane + 32, ...; the visible keys are visited in order with an fp32 online softmax.  Rows that are not visible are
-// never read, nor are the table entries of pages without a visible row, so freed pages may be anything.
+// never read, nor are the table entries of pages without a visible row, so freed pages may be anything.  It is for shapes that the tiled
+// kernels do not take, and bound by reading every row once per query and head: 256 single tokens with a window of 4,096 at 32/8 x 128 in bf16
+// 12,301 us (clusters: 315), 64 with 500 at 16/4 x 64 in fp32 672 (14.3).
 #include "window_attention.cuh"
 
 namespace b200 {

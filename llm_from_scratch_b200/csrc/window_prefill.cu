@@ -16,6 +16,16 @@
 // Tensor memory per problem: two score buffers of 64 columns (bf16 P overwrites the first half of its buffer and is the A operand of
 // O += P.V) and O.  Scores are issued a tile ahead, O is rescaled lazily, and the exponentials of the two problems take turns (see there).
 //
+// At head size 64 a problem has a CTA of its own, and two CTAs share an SM (portions below: 45 us; two problems in one CTA 48).
+//
+// Measured: 4 prompts of 8,192 at 32/8 x 128, window 4,096, 1.65 TFLOP: 1,570 .. 1,820 us, 0.91 .. 1.05 PFLOP/s with the clock under the power cap.
+// Bound by the exponentials, 16 a clock and SM.  Without the turns 1,747 us against 1,618 in the same minute; a quarter of the exponentials by
+// polynomial 1,765, half 2,064.  24 portions of 1 .. 1,000 tokens, 3,930 in all, behind up to 8,000, 16/4 x 64, window 1,024: 45 us (a warp per
+// row: 10,886), two rounds of CTAs whose rows pass 18 tiles one after the other: 1,400 cycles a tile (wait 250, scores and maximum 360,
+// exponentials 650, of which the unit needs 512), 5,000 before the first and 2,000 behind the last.
+//
+// P is rounded to bf16, the type that the tensor cores take beside bf16 values: 2^-8 of a weight.  Sums of weights are taken before that, in fp32.
+//
 // Boxes whose keys no row of the CTA sees are not read: their coordinate lies behind the pool, where a copy delivers zeros.  What is
 // left are keys that some rows see and others do not.  Their scores become -inf in the other rows, but a weight of 0 would still turn an
 // infinity or NaN of the value row into a NaN: tiles in which some row is cut are searched for one, and a CTA that finds one
