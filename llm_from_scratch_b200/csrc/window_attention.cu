@@ -97,7 +97,7 @@ int launch_general(const WindowArgs& a, int max_seqlen_q, cudaStream_t s) {
 
 int check(const WindowArgs& a, int32_t dtype) {
   if (a.num_seqs < 0 || a.Hq <= 0 || a.Hkv <= 0 || a.Hq % a.Hkv != 0 || a.D <= 0 || a.Dv <= 0 || a.bs <= 0 || a.num_blocks < 0 ||
-      a.bt_width <= 0 || a.bt_stride < 0 || a.window < 1 || a.first < 0)
+      (a.num_seqs > 0 && a.bt_width <= 0) || a.bt_stride < 0 || a.window < 1 || a.first < 0)
     return B200_ERR_ARG;
   if (dtype != B200_DTYPE_F32 && dtype != B200_DTYPE_BF16) return B200_ERR_UNSUPPORTED;
   if (a.D > 1024 || a.Dv > 1024) return B200_ERR_UNSUPPORTED;

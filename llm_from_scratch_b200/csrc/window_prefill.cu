@@ -549,7 +549,7 @@ int window_prefill_launch(const WindowArgs& a, int64_t total_q, cudaStream_t s) 
   if (a.bs < 8 || (a.bs % BN != 0 && BN % a.bs != 0)) return B200_ERR_UNSUPPORTED;
   const int64_t rows = a.num_blocks * a.bs;
   if (rows <= 0 || rows > 2147483647LL) return B200_ERR_UNSUPPORTED;       // coordinates of a copy are 32-bit
-  if (!aligned16(a.q) || a.q_stride % 8 != 0 || !aligned16(a.kc) || !aligned16(a.vc) || !aligned16(a.out)) return B200_ERR_UNSUPPORTED;
+  if (!aligned16(a.q) || a.q_stride % 8 != 0 || (total_q > 1 && a.q_stride < static_cast<int64_t>(a.Hq) * a.D) || !aligned16(a.kc) || !aligned16(a.vc) || !aligned16(a.out)) return B200_ERR_UNSUPPORTED;
   PromptArgs p{a, G, BM / G, a.bs < BN ? a.bs : BN};
   const int problems = a.D == 64 ? 1 : 2;
   const int64_t ctas = (total_q / (problems * p.tokens) + a.num_seqs) * a.Hkv;     // tiles of all portions, the last of each perhaps short

@@ -76,7 +76,8 @@ def test_ids_outside_the_pool_are_left_out_and_reported():
 
 def plain_compact(tables, pages):
     used = sorted(set(x for x in tables.flatten().tolist() if 0 <= x < pages))
-    holes = [p for p in range(len(used)) if p not in set(used)]
+    named = set(used)
+    holes = [p for p in range(len(used)) if p not in named]
     names = {p: p for p in used if p < len(used)}
     moves = list(zip([p for p in used if p >= len(used)], holes))
     names.update(moves)
@@ -161,3 +162,36 @@ def test_captured_and_on_two_streams():
         for a, b in zip(renamed[:, 19].tolist(), (perm[200:206] % 100 + 400).tolist()):
             want[b] = want[a]
         assert torch.equal(r.block_tables.cpu(), renamed) and torch.equal(pools[0], want)
+
+
+@pytest.mark.parametrize("pages,rows,width", [(70000, 300, 10), (3000, 300, 300), (65000, 300, 300), (66000, 1, 66000)])
+def test_compact_of_many_pages_or_entries(pages, rows, width):
+    from llm_from_scratch_b200 import ops
+    pools = cache([((2, 1, 4), torch.int8), ((3,), torch.float32)], pages)
+    g = torch.Generator().manual_seed(pages)
+    tables = torch.randint(-pages // 2, pages, (rows, width), generator=g).int()
+    renamed, page_map, counts, moves = plain_compact(tables, pages)
+    want = [p.clone() for p in pools]
+    at = torch.tensor(moves, dtype=torch.int64).view(-1, 2).cuda()
+    for w, p in zip(want, pools):
+        w[at[:, 1]] = p[at[:, 0]]
+    r = ops.compact_pages(ops.PagePools(pools), tables.cuda())
+    assert torch.equal(r.block_tables.cpu(), renamed) and torch.equal(r.page_map.cpu(), page_map) and r.counts.tolist() == counts
+    assert all(torch.equal(w, p) for w, p in zip(want, pools))
+    ops.check_status()
+
+
+def test_pools_beyond_32_bits():
+    from llm_from_scratch_b200 import ops
+    pool = torch.empty(70000, 65536, dtype=torch.int8, device="cuda")                       # 4.6 GB
+    page = lambda x: torch.full((65536,), x, dtype=torch.int8, device="cuda")
+    for i, x in ((69999, 1), (69998, 2), (3, 3), (0, 4)):
+        pool[i] = page(x)
+    handle = ops.PagePools([pool])
+    ids = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")
+    ops.copy_pages(handle, ids(69999, 3), ids(5, 69997))
+    assert torch.equal(pool[5], page(1)) and torch.equal(pool[69997], page(3))
+    r = ops.compact_pages(handle, ids(69998, 0, 69997, -1, 69999).view(1, 5))
+    assert r.block_tables.tolist() == [[2, 0, 1, -1, 3]] and r.counts.tolist() == [4, 3]
+    assert all(torch.equal(pool[i], page(x)) for i, x in ((0, 4), (1, 3), (2, 2), (3, 1)))
+    ops.check_status()

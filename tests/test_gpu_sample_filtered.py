@@ -252,3 +252,16 @@ def test_vocabularies_beyond_a_cluster(dtype):
     k, p, m = filters(n, vocab, g, 5000)
     for kk, pp, mm in ((k, p, m), (k, None, None), (None, p, None), (None, None, m), (None, None, None)):
         assert torch.equal(call(x, u, t, kk, pp, mm), expect(x, u, t, kk, pp, mm))
+
+
+@pytest.mark.parametrize("n,vocab", [(70000, 33000), (20000, 131072)])
+def test_rows_beyond_32_bits(n, vocab):
+    """Logits behind 2^31 elements: the tokens of the same rows alone."""
+    from llm_from_scratch_b200 import ops
+    g = torch.Generator("cuda").manual_seed(n)
+    x = torch.empty(n, vocab, dtype=torch.bfloat16, device="cuda").normal_(generator=g).mul_(4)
+    u, t, p = (torch.rand(n, generator=g, device="cuda") for _ in range(3))
+    t += 0.3
+    got = ops.sample_filtered(x, u, t, None, p, None)
+    for part in (slice(0, 40), slice(n // 2, n // 2 + 40), slice(n - 40, n)):
+        assert torch.equal(got[part], ops.sample_filtered(x[part], u[part], t[part], None, p[part], None))

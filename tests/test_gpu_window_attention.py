@@ -270,3 +270,63 @@ def test_empty_calls():
     assert ops.window_decode(q, k, k, none, torch.zeros(0, dtype=torch.int64, device="cuda"), 1.0, 5).shape == (0, 2, 64)
     cu = torch.zeros(4, dtype=torch.int32, device="cuda")
     assert ops.window_attention(q, k, k, none.expand(0, 1).new_zeros(3, 1), cu, cu, 0, 1.0, 5, 2).shape == (0, 2, 64)
+    none = torch.zeros(0, 0, dtype=torch.int32, device="cuda")
+    assert ops.window_decode(q, k, k, none, torch.zeros(0, dtype=torch.int64, device="cuda"), 1.0, 5).shape == (0, 2, 64)
+    assert ops.window_attention(q, k, k, none, cu[:1], cu[:1], 0, 1.0, 5, 2).shape == (0, 2, 64)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D", [128, 72])
+def test_pools_beyond_32_bits(D, dtype):
+    """Pages behind 2^31 elements (2^32 bytes and more): the same bits as from a small pool of those pages."""
+    from llm_from_scratch_b200 import ops
+    page, Hq, Hkv, few = 16, 16, 8, 300
+    blocks = 2 ** 31 // (page * Hkv * D) + few
+    gen = torch.Generator("cuda").manual_seed(D)
+    big = [torch.empty(blocks, page, Hkv, D, dtype=dtype, device="cuda") for _ in range(2)]
+    small = [torch.randn(few, page, Hkv, D, generator=gen, device="cuda").to(dtype) for _ in range(2)]
+    for b, s in zip(big, small):
+        b[blocks - few:] = s
+    lens = [700, 33, 1500, 16]
+    ids = torch.randperm(few, generator=gen, device="cuda")[:4 * 75].int().view(4, 75)
+    bt = torch.nn.functional.pad(ids, (0, 25), value=-1)
+    bt[2] = torch.randint(0, few, (100,), generator=gen, device="cuda")
+    far = torch.where(bt >= 0, bt + (blocks - few), bt)
+    q = torch.randn(4, Hq, D, generator=gen, device="cuda").to(dtype)
+    cl = torch.tensor(lens, device="cuda")
+    decode = lambda pools, t: ops.window_decode(q, *pools, t, cl, 0.1, 200, 3)
+    assert torch.equal(decode(big, far), decode(small, bt))
+    new = [100, 33, 129, 1]
+    cu = lambda x: torch.tensor([0] + x, device="cuda").cumsum(0).int()
+    x = torch.randn(sum(new), Hq, D, generator=gen, device="cuda").to(dtype)
+    prompts = lambda pools, t: ops.window_attention(x, *pools, t, cu(new), cu(lens), max(new), 0.1, 200, 3)
+    assert torch.equal(prompts(big, far), prompts(small, bt))
+    ops.check_status()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D", [64, 128])
+def test_token_strides_and_alignment(D, dtype):
+    """Queries inside a wider tensor, one row for all tokens, rows and pools at odd addresses."""
+    from llm_from_scratch_b200 import ops
+    gen = torch.Generator().manual_seed(D)
+    n, before, Hq, Hkv, page, window, first = 70, 50, 4, 2, 16, 33, 5
+    k, v, bt, rows = paged([n + before], page, window, first, [max(0, before + 1 - window)], gen, dtype, Hkv, D, D)
+    row = torch.randn(1, Hq, D, generator=gen).to(dtype)
+    cu = lambda x: torch.tensor([0, x], dtype=torch.int32, device="cuda")
+    shift = lambda t: torch.cat([torch.zeros(1, dtype=dtype), t.flatten()]).cuda()[1:].view(t.shape)
+    def call(q, kk, vv):
+        return ops.window_attention(q, kk, vv, bt.cuda(), cu(n), cu(n + before), n, D ** -0.5, window, first)
+    want = formula(row.expand(n, Hq, D), *rows[0], before, D ** -0.5, window, first)
+    check_close(call(row.cuda().expand(n, Hq, D), k.cuda(), v.cuda()), *want, dtype)
+    x = torch.randn(n, Hq, D, generator=gen).to(dtype)
+    want = formula(x, *rows[0], before, D ** -0.5, window, first)
+    for extra, at in ((0, 0), (8, 0), (8, 8), (3, 1), (1, 0)):
+        wide = torch.zeros(n, Hq * D + extra, dtype=dtype)
+        wide[:, at:at + Hq * D] = x.flatten(1)
+        check_close(call(wide.cuda()[:, at:at + Hq * D].unflatten(1, (Hq, D)), k.cuda(), v.cuda()), *want, dtype)
+    check_close(call(x.cuda(), shift(k), shift(v)), *want, dtype)
+    one = torch.tensor([n + before], device="cuda")
+    want = formula(x[-1:], *rows[0], n + before - 1, D ** -0.5, window, first)
+    check_close(ops.window_decode(shift(x[-1:]), shift(k), shift(v), bt.cuda(), one, D ** -0.5, window, first), *want, dtype)
+    ops.check_status()
