@@ -17,7 +17,9 @@
 // found by sums over the threads' runs.  Many long rows go through sample_wide.cu.  Histograms hold a weight in three parts of 16 bits or more, each a 32-bit counter: shared memory adds
 // 32 bits at a time.
 //
-// Bound by the reads for large rows in principle; in fact by the weights (ten 64-bit operations each) and the histogram's additions.
+// Bound by the reads for large rows in principle; in fact by the weights (ten 64-bit operations each), the histogram's additions and the cluster's
+// barriers: a row of 32,000 under all filters 15 us, 64 rows 24 .. 29 us (the first kernel, a CTA per row that read the logits for every byte of
+// a border: 199 and 270).
 #include <cooperative_groups.h>
 
 #include "sampling.cuh"
@@ -533,12 +535,12 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, const int row, u
     const bool busy = tid * words < share;
     uint32_t* own_count = &sh.upper[0][0] + tid * words * 2;       // of the share's bins
     int counted = 0;
-    float mass = 0.f, spread = 0.f;                      // by the bins' middles, and the variance of that for values anywhere in a bin
-    auto weight_of_bin = [&](int b) { return b == 0 ? 1.f : b < kBins - 1 ? fast_exp2(-1.4426950408889634f / kPerUnit * (b - 0.5f)) : 0.f; };
-    auto spread_of = [&](int b, int n, float g) {
-      // bf16 logits lie on a grid, so all of a bin may lie at one end of it: half its width for each; fp32: 1 / sqrt(12) of it, at random
-      const float e = g * (1.f / kPerUnit) * (sizeof(T) == 2 ? 0.51f * n : 0.29f), f = sizeof(T) == 2 ? e : e * e * n;
-      return b == 0 ? 0.f : f;
+    float mass = 0.f, spread = 0.f;                      // by where the bins' tokens lie on the average, and the variance of that
+    const BinPlaces<sizeof(T) == 2> places(top, step);
+    auto weight_of_bin = [&](int b, float& variance) {
+      const float g = b < kBins - 1 ? fast_exp2(-1.4426950408889634f / kPerUnit * places.of(b, variance)) : 0.f;
+      variance *= g * g * (1.f / (kPerUnit * kPerUnit));
+      return g;
     };
 #pragma unroll 1
     for (int c = 0; c < words && busy; ++c) {
@@ -550,9 +552,10 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, const int row, u
       own_count[2 * c] = lo, own_count[2 * c + 1] = hi;
       counted += lo + hi;
       const int b = 2 * (word0 + c);
-      const float g0 = weight_of_bin(b), g1 = weight_of_bin(b + 1);
+      float v0, v1;
+      const float g0 = weight_of_bin(b, v0), g1 = weight_of_bin(b + 1, v1);
       mass += lo * g0 + hi * g1;
-      spread += spread_of(b, lo, g0) + spread_of(b + 1, hi, g1);
+      spread += lo * v0 + hi * v1;
     }
     // running sums over the cluster's threads, inclusive, and the whole
     int upto = warp_upto(counted);
@@ -591,18 +594,19 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, const int row, u
 #pragma unroll 1
         for (int c = 0; c < 2 * words; ++c) {
           const int b = 2 * word0 + c, here = own_count[c];
-          const float g = weight_of_bin(b);
+          float variance;
+          const float g = weight_of_bin(b, variance);
           if (n + here >= k) {
 #pragma unroll 1
             for (int r = 0; r < ranks; ++r) {
               RowShared* to = w.other(r);
               to->bin_k = b, to->left_k = k - n, to->count_k = here;
-              to->mass_k = m + (k - n) * g, to->spread_k = e + spread_of(b, k - n, g);
+              to->mass_k = m + (k - n) * g, to->spread_k = e + (k - n) * variance;
             }
             break;
           }
           n += here;
-          m += here * g, e += spread_of(b, here, g);
+          m += here * g, e += here * variance;
         }
       }
       w.sync();
@@ -613,11 +617,12 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, const int row, u
     int listed = count_k;                                // tokens of the list
     if (nucleus) {
       // 3.5 standard deviations: a row whose border lies outside, or whose bracket has more tokens than the list takes, finds it by the histograms
-      // of weights.  Mean of 20 calls of 64 rows of 32,000, all filters: 28.6 us; with four 29.1, with five and 1e-4 31.2
+      // of weights.  Mean of 20 calls of 64 rows of 32,000, all filters: 28.6 us; with four 29.1, with five and 1e-4 31.2.
+      // bf16, top-p: 26 .. 34 us; with the bins' middles and half a bin for each token as the bound 48 .. 65
       auto off = [&](float m, float e) {
         float root;
         asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(root) : "f"(e));
-        return sizeof(T) == 2 ? e + 1e-5f * m : 3.5f * root + 1e-5f * m;
+        return 3.5f * root + 1e-5f * m;
       };
       const float goal = p * mass_all, wide = p * off(mass_all, spread_all);
       if (busy && mass_up + off(mass_up, spread_up) + wide >= goal && !(mass_up - mass - off(mass_up - mass, spread_up - spread) - wide >= goal)) {
@@ -628,8 +633,9 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, const int row, u
 #pragma unroll 1
         for (int c = 0; c < 2 * words; ++c) {
           const int b = 2 * word0 + c, here = own_count[c];
-          const float g = weight_of_bin(b);
-          m += here * g, e += spread_of(b, here, g);
+          float variance;
+          const float g = weight_of_bin(b, variance);
+          m += here * g, e += here * variance;
           const bool lo1 = m + off(m, e) + wide >= goal, hi1 = m - off(m, e) - wide >= goal;
           const bool new_lo = lo1 && !lo, new_hi = hi1 && !hi;
           if (new_lo || new_hi)
@@ -974,10 +980,10 @@ __global__ void __launch_bounds__(kThreads) sample_filtered_kernel(const SampleA
 bool fits_cluster(int vocab) { return row_smem(vocab, 8) <= 226 * 1024 && row_shape(vocab, 8).slice < 65536; }
 
 // Whether passes of separate launches are faster than clusters.  Measured (us, clusters / passes, top-p and fp32 unless told otherwise, means over
-// eight draws): 16 rows of 131,072 42 / 35, 32 49 / 39, 64 71 / 52, 256 341 / 159, 256 of bf16 480 / 169; 16 rows of 262,144 72 / 40; 64 rows of
-// 65,536 42 / 39; with all filters 64 rows of 32,000 27 / 35, 256 55 / 57, top-p alone 512 109 / 95, 256 of bf16 88 / 81; 512 rows of 16,384
-// 61 / 69, of 8,192 45 / 57; without filters 512 rows of 32,000 47 / 60, 256 of 131,072 106 / 99.  Below 65,536 tokens neither is much ahead,
-// and the passes take the host 14 us longer to launch and need a workspace.  They lose at bf16 with a small k: 64 rows of 131,072 60 / 72.
+// eight draws): 16 rows of 131,072 43 / 34, 32 50 / 39, 64 72 / 51, 256 291 / 153, 256 of bf16 247 / 144; 16 rows of 262,144 73 / 40; 64 rows of
+// 65,536 43 / 39, 128 of bf16 63 / 62; with all filters 64 rows of 32,000 28 / 35, 256 56 / 56, top-p alone 512 111 / 94, 256 of bf16 62 / 65;
+// 512 rows of 16,384 61 / 68, of 8,192 44 / 56; without filters 512 rows of 32,000 47 / 59, 256 of 131,072 107 / 98.  Below 65,536 tokens neither
+// is much ahead, and the passes take the host 14 us longer to launch and need a workspace.
 bool wide_is_faster(int64_t rows, int vocab) {
   return fits_cluster(vocab) && sample_wide_takes(rows, vocab) && vocab >= 65536 && rows * vocab >= (int64_t(1) << 22);
 }

@@ -8,10 +8,9 @@
 //   draw     a CTA per row: the list in order, the borders, the 1,024 tokens in which the draw falls, the token
 //
 // The form in shared memory reads the logits once but passes six barriers of a cluster, with two CTAs on an SM to fill the waits: 256 rows of
-// 131,072 take it 341 us.  Here they are read three times and nothing waits inside a pass: 142 us (top 25, count 33, bracket 9, sum 71, draw 17,
+// 131,072 take it 290 us.  Here they are read three times and nothing waits inside a pass: 142 us (top 25, count 33, bracket 9, sum 71, draw 17,
 // the others 4; a read alone takes 21).  Bound by the weights of the sum: ten 64-bit operations for a token that has one, of which an SM
-// does few at a time.  In bf16 175 us: its logits lie on a grid that meets the bins anywhere, so the places in the bins are added up beside the
-// counts (with the bins' middles alone the lists overflow and rows go to the other form: 280).
+// does few at a time.  In bf16 140 .. 150 us (with the bins' middles for where their tokens lie the lists overflow and rows go to the other form: 280).
 // Rows that this form does not take (greedy ones, infinite logits, u <= 0, lists that overflow, a bracket that does not hold the border) are
 // named in a list, and the other form's kernel runs over that list at the end.
 #include "sampling.cuh"
@@ -43,7 +42,6 @@ struct Wide {
   int count_tokens, sum_slices;                           // of a CTA of the two long passes
   uint32_t* slice_top;                                    // [rows, slices] order keys
   uint32_t* hist;                                         // [rows, kBins]
-  uint32_t* places;                                       // [rows, kBins]: sums of where in a bin its tokens lie, 1 / 256 of it from its far end
   RowState* state;                                        // [rows]
   unsigned long long* list_key;                           // [rows, kList]
   unsigned long long* list_mass;
@@ -97,10 +95,8 @@ __global__ void __launch_bounds__(kThreads) wide_top_kernel(const Wide w) {
     if (tid == 0) w.slice_top[row * w.slices + slice] = all;
   }
   // what the next passes add to
-  for (int i = slice * kThreads + tid; i < kBins / 4; i += w.slices * kThreads) {
+  for (int i = slice * kThreads + tid; i < kBins / 4; i += w.slices * kThreads)
     reinterpret_cast<uint4*>(w.hist + static_cast<int64_t>(row) * kBins)[i] = make_uint4(0, 0, 0, 0);
-    if (sizeof(T) == 2) reinterpret_cast<uint4*>(w.places + static_cast<int64_t>(row) * kBins)[i] = make_uint4(0, 0, 0, 0);
-  }
   if (slice == 0 && tid == 0) {
     w.state[row].list_size = w.state[row].skip = 0;
     if (row == 0) w.others[0] = 0;
@@ -145,9 +141,6 @@ __device__ __forceinline__ RowParams row_params(const Wide& w, int row) {
 
 template <typename T>
 __global__ void __launch_bounds__(kThreads) wide_count_kernel(const Wide w) {
-  // bf16 logits lie on a grid, which meets the bins anywhere: their places in the bins are added up too
-  constexpr bool GRID = sizeof(T) == 2;
-  extern __shared__ uint32_t places[];                    // [kBins], GRID only
   __shared__ uint32_t hist[kBins / 2];                    // two counts to a word: a CTA has fewer than 65,536 tokens
   const int row = blockIdx.y, tid = threadIdx.x, V = w.a.vocab;
   const RowParams r = row_params(w, row);
@@ -155,8 +148,6 @@ __global__ void __launch_bounds__(kThreads) wide_count_kernel(const Wide w) {
   const T* x = static_cast<const T*>(w.a.logits) + row * w.a.row_stride;
   const bool wide = wide_loads(x);
   for (int i = tid; i < kBins / 2; i += kThreads) hist[i] = 0;
-  if (GRID)
-    for (int i = tid; i < kBins; i += kThreads) places[i] = 0;
   __syncthreads();
   const int last = r.k > 0 ? kBins : kBins - 1;           // what is in the last bin has no weight
   const int end = min_of((blockIdx.x + 1) * w.count_tokens, V);
@@ -166,12 +157,8 @@ __global__ void __launch_bounds__(kThreads) wide_count_kernel(const Wide w) {
     load4_raw(x, i, V, wide, v);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const float y = fminf((r.top - v[j]) * r.step, kBins - 1.f);         // NaN goes to the last bin, as do places behind the row
-      const int b = __float2int_ru(y);
-      if (b < last) {
-        atomicAdd(&hist[b & (kBins / 2 - 1)], b >= kBins / 2 ? 0x10000u : 1u);
-        if (GRID) atomicAdd(&places[b], static_cast<uint32_t>((b - y) * 256.f));
-      }
+      const int b = __float2int_ru(fminf((r.top - v[j]) * r.step, kBins - 1.f));       // NaN goes to the last bin, as do places behind the row
+      if (b < last) atomicAdd(&hist[b & (kBins / 2 - 1)], b >= kBins / 2 ? 0x10000u : 1u);
     }
   }
   __syncthreads();
@@ -180,11 +167,6 @@ __global__ void __launch_bounds__(kThreads) wide_count_kernel(const Wide w) {
     const uint32_t y = hist[i];
     if (y & 0xffff) atomicAdd(out + i, y & 0xffff);
     if (y >> 16) atomicAdd(out + kBins / 2 + i, y >> 16);
-  }
-  if (GRID) {
-    uint32_t* out_places = w.places + static_cast<int64_t>(row) * kBins;
-    for (int i = tid; i < kBins; i += kThreads)
-      if (places[i]) atomicAdd(out_places + i, places[i]);
   }
 }
 
@@ -228,31 +210,28 @@ __global__ void __launch_bounds__(kRowThreads) wide_bracket_kernel(const Wide w)
       const uint4 y = from[c];
       count[4 * c] = y.x, count[4 * c + 1] = y.y, count[4 * c + 2] = y.z, count[4 * c + 3] = y.w;
     }
-    // a bin's mass by its middle, and the variance of that for values anywhere in it (fp32); or by the mean place of its tokens, and how far off
-    // that may be (bf16): 1 / 512 of a bin, and half of the square of a bin's width for places on both sides of the mean
-    const uint32_t* places = w.places + static_cast<int64_t>(row) * kBins;
-    auto weight_of_bin = [&](int b, int n) {
-      const float back = sizeof(T) == 2 && n > 0 ? (places[b] * (1.f / 256.f)) / n + 1.f / 512.f : 0.5f;
-      return b == 0 ? 1.f : b < kBins - 1 ? fast_exp2(-1.4426950408889634f / kPerUnit * (b - back)) : 0.f;
-    };
-    auto spread_of = [&](int b, int n, float g) {
-      const float e = g * (1.f / kPerUnit) * (sizeof(T) == 2 ? 0.005f * n : 0.29f), f = sizeof(T) == 2 ? e : e * e * n;
-      return b == 0 ? 0.f : f;
+    // a bin's weight where its tokens lie on the average, and the variance of that
+    const BinPlaces<sizeof(T) == 2> places(r.top, r.step);
+    auto weight_of_bin = [&](int b, float& variance) {
+      const float g = b < kBins - 1 ? fast_exp2(-1.4426950408889634f / kPerUnit * places.of(b, variance)) : 0.f;
+      variance *= g * g * (1.f / (kPerUnit * kPerUnit));
+      return g;
     };
     // four standard deviations: a border outside costs its row the other form (75 us), as does a bracket of more tokens than the list takes.
     // Mean of 20 calls of 256 rows of 131,072, p up to 0.99: 159 us; with five and 1e-4 182 (11 rows went, not 4)
     auto off = [&](float m, float e) {
       float root;
       asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(root) : "f"(e));
-      return sizeof(T) == 2 ? e + 1e-5f * m : 4.f * root + 1e-5f * m;
+      return 4.f * root + 1e-5f * m;
     };
     int counted = 0;
     float mass = 0.f, spread = 0.f;
 #pragma unroll
     for (int c = 0; c < kOwnBins; ++c) {
       const int b = tid * kOwnBins + c;
-      const float g = weight_of_bin(b, count[c]);
-      counted += count[c], mass += count[c] * g, spread += spread_of(b, count[c], g);
+      float variance;
+      const float g = weight_of_bin(b, variance);
+      counted += count[c], mass += count[c] * g, spread += count[c] * variance;
     }
     int all;
     float mass_all, spread_all;
@@ -265,9 +244,10 @@ __global__ void __launch_bounds__(kRowThreads) wide_bracket_kernel(const Wide w)
 #pragma unroll
         for (int c = 0; c < kOwnBins; ++c) {
           const int b = tid * kOwnBins + c, here = count[c];
-          const float g = weight_of_bin(b, here);
-          if (n < r.k && n + here >= r.k) bin_k = b, left_k = r.k - n, mass_k = m + (r.k - n) * g, spread_k = e + spread_of(b, r.k - n, g);
-          n += here, m += here * g, e += spread_of(b, here, g);
+          float variance;
+          const float g = weight_of_bin(b, variance);
+          if (n < r.k && n + here >= r.k) bin_k = b, left_k = r.k - n, mass_k = m + (r.k - n) * g, spread_k = e + (r.k - n) * variance;
+          n += here, m += here * g, e += here * variance;
         }
       }
       __syncthreads();
@@ -280,8 +260,9 @@ __global__ void __launch_bounds__(kRowThreads) wide_bracket_kernel(const Wide w)
 #pragma unroll
         for (int c = 0; c < kOwnBins; ++c) {
           const int b = tid * kOwnBins + c;
-          const float g = weight_of_bin(b, count[c]);
-          m += count[c] * g, e += spread_of(b, count[c], g);
+          float variance;
+          const float g = weight_of_bin(b, variance);
+          m += count[c] * g, e += count[c] * variance;
           if (m + off(m, e) + wide >= goal) atomicMin(&bin_lo, b);
           if (m - off(m, e) - wide >= goal) atomicMin(&bin_hi, b);
         }
@@ -589,8 +570,7 @@ int launch_wide(const Wide& w, cudaStream_t s) {
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64) return B200_ERR_UNSUPPORTED;
   if (!configured[dev]) {
-    if (cudaFuncSetAttribute(wide_draw_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(DrawShared)) != cudaSuccess ||
-        cudaFuncSetAttribute(wide_count_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kBins * 4) != cudaSuccess) {
+    if (cudaFuncSetAttribute(wide_draw_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(DrawShared)) != cudaSuccess) {
       cudaGetLastError();
       return B200_ERR_LAUNCH;
     }
@@ -598,7 +578,7 @@ int launch_wide(const Wide& w, cudaStream_t s) {
   }
   wide_top_kernel<T><<<dim3(w.slices, w.rows), kThreads, 0, s>>>(w);
   if (w.a.top_k != nullptr || w.a.top_p != nullptr)
-    wide_count_kernel<T><<<dim3((w.a.vocab + w.count_tokens - 1) / w.count_tokens, w.rows), kThreads, sizeof(T) == 2 ? kBins * 4 : 0, s>>>(w);
+    wide_count_kernel<T><<<dim3((w.a.vocab + w.count_tokens - 1) / w.count_tokens, w.rows), kThreads, 0, s>>>(w);
   wide_bracket_kernel<T><<<w.rows, kRowThreads, 0, s>>>(w);
   wide_sum_kernel<T><<<dim3((w.slices + w.sum_slices - 1) / w.sum_slices, w.rows), kThreads, 0, s>>>(w);
   wide_draw_kernel<T><<<w.rows, kRowThreads, sizeof(DrawShared), s>>>(w);
@@ -611,7 +591,7 @@ size_t aligned(size_t x) { return (x + 255) & ~size_t(255); }
 
 size_t sample_wide_workspace_bytes(int64_t rows, int vocab) {
   const size_t n = rows, slices = (vocab + kSlice - 1) / kSlice, chunks = (vocab + kChunk - 1) / kChunk;
-  return aligned(n * slices * 4) + 2 * aligned(n * kBins * 4) + aligned(n * sizeof(RowState)) + 2 * aligned(n * kList * 8) + aligned(n * chunks * 24) +
+  return aligned(n * slices * 4) + aligned(n * kBins * 4) + aligned(n * sizeof(RowState)) + 2 * aligned(n * kList * 8) + aligned(n * chunks * 24) +
          aligned((n + 1) * 4);
 }
 
@@ -640,7 +620,6 @@ int sample_wide_launch(const SampleArgs& a, int64_t rows, int32_t dtype, void* w
   };
   w.slice_top = reinterpret_cast<uint32_t*>(take(n * w.slices * 4));
   w.hist = reinterpret_cast<uint32_t*>(take(n * kBins * 4));
-  w.places = reinterpret_cast<uint32_t*>(take(n * kBins * 4));
   w.state = reinterpret_cast<RowState*>(take(n * sizeof(RowState)));
   w.list_key = reinterpret_cast<unsigned long long*>(take(n * kList * 8));
   w.list_mass = reinterpret_cast<unsigned long long*>(take(n * kList * 8));

@@ -138,6 +138,32 @@ __device__ __forceinline__ void sort_by_key(unsigned long long* key, unsigned lo
     }
 }
 
+// Where the tokens of a bin lie that is told by b = ceil((top - x) step): their mean distance from the maximum in bins and its variance, if
+// all logits that the bin can hold are equally likely.  fp32: anywhere in it.  bf16 (GRID): on a grid, which meets the bins anywhere and is often
+// coarser than they are; with their middles instead, sums of weights would be off by half a bin to one side.  An estimate only: it narrows down
+// where borders lie, and what rests on it is checked with the weights.
+template <bool GRID>
+struct BinPlaces {
+  float top, step, width;
+  __device__ __forceinline__ BinPlaces(float top, float step) : top(top), step(step), width(1.f / step) {}
+  __device__ __forceinline__ float of(int b, float& variance) const {
+    variance = b == 0 ? 0.f : 1.f / 12.f;
+    if (!GRID || b == 0) return b == 0 ? 0.f : b - 0.5f;
+    const float middle = top - (b - 0.5f) * width;
+    const float grain = fmaxf(__uint_as_float(__float_as_uint(middle) & 0x7f800000u) * 0.0078125f, 1e-30f), per = 1.f / grain;
+    auto bin = [&](float x) { return ceilf((top - x) * step); };
+    float high = floorf((top - (b - 1) * width) * per) * grain, low = ceilf((top - b * width) * per) * grain;
+    if (bin(high) < b) high -= grain;
+    else if (bin(high + grain) == b) high += grain;
+    if (bin(low) > b) low += grain;
+    else if (bin(low - grain) == b) low -= grain;
+    if (!(low <= high)) low = high = rintf(middle * per) * grain;          // none: the next one
+    const float n = (high - low) * per + 1.f, apart = grain * step;
+    variance = apart * apart * (n * n - 1.f) * (1.f / 12.f);
+    return fminf(fmaxf((top - 0.5f * (high + low)) * step, b - 1.f), static_cast<float>(b));
+  }
+};
+
 // Many long rows (sample_wide.cu): rows that it leaves to the other form are named in `others`, their number first.
 size_t sample_wide_workspace_bytes(int64_t rows, int vocab);
 bool sample_wide_takes(int64_t rows, int vocab);
