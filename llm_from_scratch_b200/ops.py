@@ -1808,11 +1808,9 @@ def compact_pages(pools: PagePools, block_tables: torch.Tensor) -> CompactedPage
     if stride < width:
         raise ValueError("block_tables rows must not overlap")
     n = pools.num_pages
-    tables = torch.empty((rows, width), dtype=torch.int32, device=dev)
-    page_map = torch.empty(n, dtype=torch.int32, device=dev)
-    counts = torch.empty(2, dtype=torch.int32, device=dev)
-    moves = torch.empty(2 * n, dtype=torch.int32, device=dev)
-    check(lib.b200_compact_pages(*pools._args, block_tables.data_ptr(), stride, rows, width, tables.data_ptr(), page_map.data_ptr(),
-                                 moves.data_ptr(), moves.data_ptr() + 4 * n, counts.data_ptr(), status_word(dev).data_ptr(), _stream()),
-          "compact_pages")
-    return CompactedPages(tables, page_map, counts)
+    tables = block_tables.new_empty((rows, width))
+    plan = block_tables.new_empty(3 * n + 2)                        # the map, the counts, the moves: one allocation instead of three
+    at = plan.data_ptr()
+    check(lib.b200_compact_pages(*pools._args, block_tables.data_ptr(), stride, rows, width, tables.data_ptr(), at, at + 4 * n + 8,
+                                 at + 8 * n + 8, at + 4 * n, status_word(dev).data_ptr(), _stream()), "compact_pages")
+    return CompactedPages(tables, plan[:n], plan[n:n + 2])
