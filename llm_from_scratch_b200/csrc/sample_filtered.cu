@@ -18,7 +18,7 @@
 // 32 bits at a time.
 //
 // Bound by the reads for large rows in principle; in fact by the weights (ten 64-bit operations each), the histogram's additions and the cluster's
-// barriers: a row of 32,000 under all filters 15 us, 64 rows 24 .. 29 us (the first kernel, a CTA per row that read the logits for every byte of
+// barriers: a row of 32,000 under all filters 15 us, 64 rows 25 us (the first kernel, a CTA per row that read the logits for every byte of
 // a border: 199 and 270).
 #include <cooperative_groups.h>
 
@@ -616,13 +616,14 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, const int row, u
     int bin_lo = kBins, bin_hi = kBins - 1;              // bins among which the nucleus ends
     int listed = count_k;                                // tokens of the list
     if (nucleus) {
-      // 3.5 standard deviations: a row whose border lies outside, or whose bracket has more tokens than the list takes, finds it by the histograms
-      // of weights.  Mean of 20 calls of 64 rows of 32,000, all filters: 28.6 us; with four 29.1, with five and 1e-4 31.2.
-      // bf16, top-p: 26 .. 34 us; with the bins' middles and half a bin for each token as the bound 48 .. 65
+      // One standard deviation of the sum in front, and one of p times the whole, which in part is the same sum: with the bins' own widths a border
+      // is seldom outside.  Such a row, and one whose bracket has more tokens than the list takes, finds it by the histograms of weights.  Means of
+      // 20 calls (us) at 3.5, 2, 1.2 and 0.6 deviations: 64 rows of 32,000, all filters, 28.8, 26.6, 25.6, 24.7; 256 with top-p 69, 63, 61, 59; 64
+      // of bf16 with top-p 36.8, 31.7, 29.6, 30.1 (with the bins' middles and half a bin for each token as the bound: 48 .. 65)
       auto off = [&](float m, float e) {
         float root;
         asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(root) : "f"(e));
-        return 3.5f * root + 1e-5f * m;
+        return root + 1e-5f * m;
       };
       const float goal = p * mass_all, wide = p * off(mass_all, spread_all);
       if (busy && mass_up + off(mass_up, spread_up) + wide >= goal && !(mass_up - mass - off(mass_up - mass, spread_up - spread) - wide >= goal)) {
@@ -980,10 +981,11 @@ __global__ void __launch_bounds__(kThreads) sample_filtered_kernel(const SampleA
 bool fits_cluster(int vocab) { return row_smem(vocab, 8) <= 226 * 1024 && row_shape(vocab, 8).slice < 65536; }
 
 // Whether passes of separate launches are faster than clusters.  Measured (us, clusters / passes, top-p and fp32 unless told otherwise, means over
-// eight draws): 16 rows of 131,072 43 / 34, 32 50 / 39, 64 72 / 51, 256 291 / 153, 256 of bf16 247 / 144; 16 rows of 262,144 73 / 40; 64 rows of
-// 65,536 43 / 39, 128 of bf16 63 / 62; with all filters 64 rows of 32,000 28 / 35, 256 56 / 56, top-p alone 512 111 / 94, 256 of bf16 62 / 65;
-// 512 rows of 16,384 61 / 68, of 8,192 44 / 56; without filters 512 rows of 32,000 47 / 59, 256 of 131,072 107 / 98.  Below 65,536 tokens neither
-// is much ahead, and the passes take the host 14 us longer to launch and need a workspace.
+// eight draws): 16 rows of 131,072 33 / 34, 32 40 / 38, 64 67 / 51, 256 251 / 142, 256 of bf16 247 / 144; 16 rows of 262,144 60 / 39; 64 rows of
+// 65,536 37 / 38, 128 of bf16 63 / 62; with all filters 64 rows of 32,000 25 / 35, 256 55 / 56, top-p alone 512 104 / 94, 256 of bf16 63 / 65;
+// 512 rows of 16,384 55 / 68, of 8,192 40 / 56; without filters 512 rows of 32,000 47 / 60, 256 of 131,072 107 / 99; with a small k 32 rows of
+// 131,072 in bf16 33 / 52, 64 63 / 65.  Below 65,536 tokens the passes are not much ahead anywhere, take the host 14 us longer to launch and need a
+// workspace.
 bool wide_is_faster(int64_t rows, int vocab) {
   return fits_cluster(vocab) && sample_wide_takes(rows, vocab) && vocab >= 65536 && rows * vocab >= (int64_t(1) << 22);
 }

@@ -8,7 +8,7 @@
 //   draw     a CTA per row: the list in order, the borders, the 1,024 tokens in which the draw falls, the token
 //
 // The form in shared memory reads the logits once but passes six barriers of a cluster, with two CTAs on an SM to fill the waits: 256 rows of
-// 131,072 take it 290 us.  Here they are read three times and nothing waits inside a pass: 142 us (top 25, count 33, bracket 9, sum 71, draw 17,
+// 131,072 take it 251 us.  Here they are read three times and nothing waits inside a pass: 142 us (top 25, count 33, bracket 9, sum 71, draw 17,
 // the others 4; a read alone takes 21).  Bound by the weights of the sum: ten 64-bit operations for a token that has one, of which an SM
 // does few at a time.  In bf16 140 .. 150 us (with the bins' middles for where their tokens lie the lists overflow and rows go to the other form: 280).
 // Rows that this form does not take (greedy ones, infinite logits, u <= 0, lists that overflow, a bracket that does not hold the border) are
@@ -217,12 +217,12 @@ __global__ void __launch_bounds__(kRowThreads) wide_bracket_kernel(const Wide w)
       variance *= g * g * (1.f / (kPerUnit * kPerUnit));
       return g;
     };
-    // four standard deviations: a border outside costs its row the other form (75 us), as does a bracket of more tokens than the list takes.
-    // Mean of 20 calls of 256 rows of 131,072, p up to 0.99: 159 us; with five and 1e-4 182 (11 rows went, not 4)
+    // 1.2 standard deviations (as there): a border outside costs its row the other form (75 us), as does a bracket of more tokens than the list
+    // takes.  Means of 20 calls of 256 rows of 131,072, p up to 0.99: 142 us; with two 147, with 3.5 159
     auto off = [&](float m, float e) {
       float root;
       asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(root) : "f"(e));
-      return 4.f * root + 1e-5f * m;
+      return 1.2f * root + 1e-5f * m;
     };
     int counted = 0;
     float mass = 0.f, spread = 0.f;
