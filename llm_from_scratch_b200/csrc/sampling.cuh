@@ -150,7 +150,8 @@ struct BinPlaces {
     variance = b == 0 ? 0.f : 1.f / 12.f;
     if (!GRID || b == 0) return b == 0 ? 0.f : b - 0.5f;
     const float middle = top - (b - 0.5f) * width;
-    const float grain = fmaxf(__uint_as_float(__float_as_uint(middle) & 0x7f800000u) * 0.0078125f, 1e-30f), per = 1.f / grain;
+    const uint32_t exponent = max(__float_as_uint(middle) & 0x7f800000u, 0x10000000u) - (7u << 23);      // eight bits of a number
+    const float grain = __uint_as_float(exponent), per = __uint_as_float(0x7f000000u - exponent);        // a power of two and its reciprocal
     auto bin = [&](float x) { return ceilf((top - x) * step); };
     float high = floorf((top - (b - 1) * width) * per) * grain, low = ceilf((top - b * width) * per) * grain;
     if (bin(high) < b) high -= grain;
