@@ -19,6 +19,9 @@ def main(argv=None) -> int:
     g.add_argument("--dtype", default="bfloat16", choices=["bfloat16", "float32"])
     g.add_argument("--max-tokens", type=int, default=65, help="stop rule of the engine: max_tokens - 1 tokens are generated")
     g.add_argument("--temperature", type=float, default=0.0)
+    g.add_argument("--top-k", type=int, default=0, help="most likely tokens that are drawn from (0: all)")
+    g.add_argument("--top-p", type=float, default=1.0, help="share of the weight that the most likely tokens drawn from reach (1: all)")
+    g.add_argument("--min-p", type=float, default=0.0, help="least weight of a token, the most likely one weighing 1")
     g.add_argument("--eos", type=int, default=-1)
     g.add_argument("--ignore-eos", action="store_true")
     g.add_argument("--block-size", type=int, default=16)
@@ -39,8 +42,8 @@ def main(argv=None) -> int:
                             max_num_sequences=args.max_num_sequences, max_num_batched_tokens=args.max_num_batched_tokens,
                             max_cached_blocks=args.max_cached_blocks, max_model_length=args.max_model_length,
                             gpu_memory_utilization=0.5))
-    out = engine.generate(prompts, SamplingParams(temperature=args.temperature, max_tokens=args.max_tokens,
-                                                  ignore_eos=args.ignore_eos))
+    out = engine.generate(prompts, SamplingParams(temperature=args.temperature, max_tokens=args.max_tokens, ignore_eos=args.ignore_eos,
+                                                  top_k=args.top_k, top_p=args.top_p, min_p=args.min_p))
     for ids in out["token_ids"]:
         print(json.dumps({"token_ids": ids}))
     engine.exit()

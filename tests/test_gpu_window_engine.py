@@ -1,9 +1,15 @@
 """A decoder with a sliding window and visible first tokens through the engine: against a plain restatement in 64 bits, with pages given back
 behind the window, forks of running sequences and filtered sampling, one by one and together."""
 import itertools
+import json
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
+
+from engine_helpers import write_model
 
 pytestmark = pytest.mark.gpu
 CFG = dict(vocab_size=97, context_length=1024, d_model=256, num_layers=2, num_heads=4, num_kv_heads=2, d_ff=96, attention_type="GQA",
@@ -187,3 +193,21 @@ def test_all_together(eager, dtype):
     assert all(a != b for a, b in pairs)                                                      # they draw on their own
     assert eng.scheduler.block_manager.num_free_blocks == 60
     eng.exit()
+
+
+@pytest.mark.parametrize("options,keep", [(["--temperature", "0.8", "--top-k", "1"], 1), (["--temperature", "2", "--top-k", "3", "--top-p", "0.9", "--min-p", "0.01"], 3)])
+def test_generate_command_line(tmp_path, options, keep):
+    w = weights()
+    write_model(tmp_path / "m", CFG, w)
+    prompts = [PROMPTS[2], PROMPTS[4]]
+    r = subprocess.run([sys.executable, "-m", "llm_from_scratch_b200", "generate", "--model", str(tmp_path / "m"), "--dtype", "float32",
+                        "--max-tokens", "31", "--max-model-length", "1024", "--max-cached-blocks", "64", "--ignore-eos"] + options
+                       + [" ".join(map(str, p)) for p in prompts],
+                       capture_output=True, text=True, timeout=300, cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
+    assert r.returncode == 0, r.stderr[-2000:]
+    for prompt, line in zip(prompts, r.stdout.splitlines(), strict=True):
+        got = json.loads(line)["token_ids"]
+        logits = restate(prompt + got, w)[len(prompt) - 1:-1]
+        assert len(got) == 30
+        chosen = logits.gather(1, torch.tensor(got)[:, None])[:, 0]
+        assert (logits.topk(keep, -1).values[:, -1] - chosen).max() <= SLACK[torch.float32] * logits.std()
