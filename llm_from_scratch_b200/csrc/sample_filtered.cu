@@ -14,8 +14,8 @@
 // A cluster of CTAs shares a row, whose logits stay in shared memory: a thread owns a run of neighbouring tokens.  Borders by value (top-k with
 // ones as masses, top-p with the weights) are found with a histogram over the distance from the maximum, in steps of T / 128, and, if the
 // border's bin holds more than a few tokens, over ever finer ranges of the logits' bits; what is left is sorted.  The border of the draw is
-// found by sums over the threads' runs.  Many long rows go through sample_wide.cu.  Histograms hold a weight in three parts of 16 bits or more, each a 32-bit counter: shared memory adds
-// 32 bits at a time.
+// found by sums over the threads' runs.  Many long rows go through sample_wide.cu.  Histograms hold a weight in three parts of 16 bits or more,
+// each a 32-bit counter: shared memory adds 32 bits at a time.
 //
 // Bound by the reads for large rows in principle; in fact by the weights (ten 64-bit operations each), the histogram's additions and the cluster's
 // barriers: a row of 32,000 under all filters 15 us, 64 rows 25 us (the first kernel, a CTA per row that read the logits for every byte of
@@ -530,7 +530,8 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, const int row, u
       sh.before_lo = sh.upto_hi = 0xffffffffu;
     }
     w.sync();
-    // a CTA adds up a share of the bins, a thread a run of up to four words of it, two bins each
+    // a CTA adds up a share of the bins, a thread a run of up to four words of it, two bins each.  (Where every CTA adds up all bins and
+    // finds the borders for itself, two barriers of the cluster less, a row of 32,000 takes 19.9 us against 16.5, 64 rows 25.7 against 25.3.)
     const int share = kBins / 2 / ranks, words = max_of(share / kRowThreads, 1), word0 = rank * share + tid * words;
     const bool busy = tid * words < share;
     uint32_t* own_count = &sh.upper[0][0] + tid * words * 2;       // of the share's bins
@@ -538,6 +539,7 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, const int row, u
     float mass = 0.f, spread = 0.f;                      // by where the bins' tokens lie on the average, and the variance of that
     const BinPlaces<sizeof(T) == 2> places(top, step);
     auto weight_of_bin = [&](int b, float& variance) {
+      variance = 0.f;                                    // of the last bin, which weighs nothing
       const float g = b < kBins - 1 ? fast_exp2(-1.4426950408889634f / kPerUnit * places.of(b, variance)) : 0.f;
       variance *= g * g * (1.f / (kPerUnit * kPerUnit));
       return g;
@@ -618,8 +620,8 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, const int row, u
     if (nucleus) {
       // One standard deviation of the sum in front, and one of p times the whole, which in part is the same sum: with the bins' own widths a border
       // is seldom outside.  Such a row, and one whose bracket has more tokens than the list takes, finds it by the histograms of weights.  Means of
-      // 20 calls (us) at 3.5, 2, 1.2 and 0.6 deviations: 64 rows of 32,000, all filters, 28.8, 26.6, 25.6, 24.7; 256 with top-p 69, 63, 61, 59; 64
-      // of bf16 with top-p 36.8, 31.7, 29.6, 30.1 (with the bins' middles and half a bin for each token as the bound: 48 .. 65)
+      // 20 calls (us) at 3.5, 2, 1.2 and 0.6 deviations: 64 rows of 32,000, all filters, 28.8, 26.6, 25.6, 24.7; 256 with top-p 69, 63, 61, 59.  64 of
+      // bf16 with top-p: 25.4 (with the bins' middles and half a bin for each token as the bound: 48 .. 65)
       auto off = [&](float m, float e) {
         float root;
         asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(root) : "f"(e));

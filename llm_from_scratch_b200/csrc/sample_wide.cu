@@ -213,6 +213,7 @@ __global__ void __launch_bounds__(kRowThreads) wide_bracket_kernel(const Wide w)
     // a bin's weight where its tokens lie on the average, and the variance of that
     const BinPlaces<sizeof(T) == 2> places(r.top, r.step);
     auto weight_of_bin = [&](int b, float& variance) {
+      variance = 0.f;                                    // of the last bin, which weighs nothing
       const float g = b < kBins - 1 ? fast_exp2(-1.4426950408889634f / kPerUnit * places.of(b, variance)) : 0.f;
       variance *= g * g * (1.f / (kPerUnit * kPerUnit));
       return g;
