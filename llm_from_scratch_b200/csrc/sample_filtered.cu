@@ -18,7 +18,7 @@
 // each a 32-bit counter: shared memory adds 32 bits at a time.
 //
 // Bound by the reads for large rows in principle; in fact by the weights (ten 64-bit operations each), the histogram's additions and the cluster's
-// barriers: a row of 32,000 under all filters 15 us, 64 rows 25 us (the first kernel, a CTA per row that read the logits for every byte of
+// barriers: a row of 32,000 under all filters 16 us, 64 rows 25 us (the first kernel, a CTA per row that read the logits for every byte of
 // a border: 199 and 270).
 #include <cooperative_groups.h>
 
