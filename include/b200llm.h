@@ -82,8 +82,8 @@ int64_t b200_block_hash_chain(const int32_t* token_ids_host, int64_t num_tokens,
  * handed out oldest-free-first (the reference's FIFO deque, :60-78); full blocks are sealed with the chained
  * hash above and found again by later prompts (:85-114) after a token-by-token comparison; reference counts
  * start at 1 (the reference starts at 0 and so leaks unshared blocks, :23-26; this is the engine's corrected
- * default mode), a released block keeps its contents and can be revived, and a hit never covers a whole
- * prompt.  Host-only, no GPU work; a handle is not thread-safe.
+ * default mode), a released block keeps its contents and can be revived, hits end at the first block that is not
+ * cached, and never cover a whole prompt.  Host-only, no GPU work; a handle is not thread-safe.
  *   b200_pool_allocate    blocks for a new sequence (allocate, :85-114): writes ceil(num_tokens/block_size) block
  *                         ids, *num_cached_out = tokens covered by reused blocks; returns the number of
  *                         blocks, or B200_ERR_TOO_LARGE when the pool runs dry (state partly applied, as

@@ -112,8 +112,10 @@ extern "C" int64_t b200_pool_allocate(void* pool, const int32_t* token_ids, int6
       h = b200_block_hash(toks, bs, chain ? h : 0, chain ? 1 : 0);
       chain = true;
       auto it = p->by_hash.find(h);
-      // a hit on the block that ends the prompt would leave no token to run through the model
-      if (it != p->by_hash.end() && p->has_hash[it->second] && p->hash[it->second] == h &&
+      // Hits end at the first miss: num_cached counts the prefix whose keys exist, and blocks of a prefix may be evicted before those behind
+      // them (given back behind a window, sealed a second time by a fork or by a prompt that computes its last block again).  A hit on the
+      // block that ends the prompt would leave no token to run through the model.
+      if (cached == i * bs && it != p->by_hash.end() && p->has_hash[it->second] && p->hash[it->second] == h &&
           p->same_tokens(it->second, toks) && cached + bs < num_tokens)
         b = it->second;
     }
