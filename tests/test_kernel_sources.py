@@ -24,3 +24,13 @@ def test_no_cta_leaves_while_its_bulk_copies_may_be_on_their_way():
     helper = helper[:helper.index("\n}\n")]
     at = [helper.index(x) for x in ("__syncthreads_or(!here)", "mbar_wait(bar", "__syncthreads();", "return false")]
     assert at == sorted(at)
+
+
+def test_no_cta_writes_to_one_of_its_cluster_that_may_not_have_started():
+    """Rows in clusters: every CTA has passed a barrier of the cluster before the first step that writes to another one's shared memory."""
+    text = (CSRC / "sample_filtered.cu").read_text()
+    body = text[text.index("void sample_row(const SampleArgs& a"):text.index("void __launch_bounds__(kRowThreads, 2) sample_row_kernel")]
+    arrive, wait = "barrier.cluster.arrive", "barrier.cluster.wait"
+    assert body.count(arrive) == 1 and body.count(wait) == 1
+    first = min(body.index(x) for x in ("combine_max(w", "combine(w", "first_highest(w", "locate(w", "cut(w", "w.sync()", "w.other("))
+    assert body.index(arrive) < body.index(wait) < first
