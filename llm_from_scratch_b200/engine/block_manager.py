@@ -261,10 +261,15 @@ class BlockManager:
 
 
 
+def blocks_to_fork(seq: Sequence, block_size: int) -> int:
+    """Blocks that a fork of ``seq`` opens: at most the one that is written to and one opened ahead."""
+    return len(seq.block_table) - min((seq.num_tokens - 1) // block_size, len(seq.block_table))
+
+
 def _fork(manager, seq: Sequence, child: Sequence, share) -> list[tuple[int, int]]:
     bs, written = manager.block_size, seq.num_tokens - 1          # the last token's keys do not exist yet
-    full = min(written // bs, len(seq.block_table))
-    own = len(seq.block_table) - full                             # at most the open block and one opened ahead
+    own = blocks_to_fork(seq, bs)
+    full = len(seq.block_table) - own
     if own > manager.num_free_blocks:
         raise IndexError("KV block pool exhausted")
     child.block_table = seq.block_table[:full]

@@ -66,16 +66,22 @@ class LLMEngine:
 
     def fork(self, seq: Sequence, n: int = 1, sampling_params: SamplingParams | None = None) -> list[Sequence]:
         """``n`` further continuations of a running sequence from the tokens it has now, under ``sampling_params`` (None: its own).
-        They share its full cache blocks; the block that is still being written is copied (``ops.copy_pages``).  Between two steps only."""
+        They share its full cache blocks; the block that is still being written is copied (``ops.copy_pages``).  Between two steps only.
+        All ``n`` or none: where the pool does not cover them, or a copy fails, the call raises and nothing runs on."""
+        if not self.scheduler.can_fork(seq, n):
+            raise IndexError("KV block pool exhausted")
         children, copies = [], []
         try:
             for _ in range(n):
                 child, pairs = self.scheduler.fork(seq, sampling_params)
                 children.append(child)
                 copies += pairs
-        finally:
             if copies:
                 self.model_runner.copy_blocks(copies)
+        except BaseException:
+            for child in children:
+                self.scheduler.drop_fork(child)
+            raise
         return children
 
     # ------------------------------------------------------------------ one step

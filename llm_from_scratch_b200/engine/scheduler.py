@@ -16,7 +16,7 @@ from __future__ import annotations
 import itertools
 from collections import deque
 
-from .block_manager import BlockManager, NativeBlockManager
+from .block_manager import BlockManager, NativeBlockManager, blocks_to_fork
 from .sequence import Sequence, SequenceStatus
 
 
@@ -205,7 +205,8 @@ class Scheduler:
 
     def fork(self, seq: Sequence, sampling_params=None) -> tuple[Sequence, list[tuple[int, int]]]:
         """A running sequence that continues from the tokens of ``seq`` on its own (``sampling_params`` None: those of ``seq``); it
-        shares the full blocks.  Returns it and the (source, target) blocks to copy before the next step."""
+        shares the full blocks.  Returns it and the (source, target) blocks to copy before the next step.  With more than
+        ``max_num_sequences`` running the newest ones wait until others end."""
         if seq.status is not SequenceStatus.RUNNING or seq not in self.running:
             raise ValueError("only a running sequence can be forked")
         child = Sequence(seq.token_ids, sampling_params)
@@ -217,6 +218,16 @@ class Scheduler:
         child.status = SequenceStatus.RUNNING
         self.running.append(child)
         return child, copies
+
+    def can_fork(self, seq: Sequence, n: int) -> bool:
+        """Whether the pool has the blocks that ``n`` forks of ``seq`` open."""
+        return n * blocks_to_fork(seq, self.block_manager.block_size) <= self.block_manager.num_free_blocks
+
+    def drop_fork(self, child: Sequence) -> None:
+        """Takes back a fork that has not run a step."""
+        self.running.remove(child)
+        self.block_manager.deallocate(child)
+        child.status = SequenceStatus.FINISHED
 
     def preempt(self, seq: Sequence) -> None:
         self.block_manager.deallocate(seq)
