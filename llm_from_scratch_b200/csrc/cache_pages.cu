@@ -144,8 +144,9 @@ __device__ __forceinline__ int block_sum_upto(int v, int* s_warp, int* total) {
 __global__ void __launch_bounds__(kPlanThreads) plan_pages_kernel(int32_t* page_map, int num_pages, int32_t* source, int32_t* target,
                                                                   int32_t* counts) {
   __shared__ int s_warp[kPlanThreads / 32];
-  const int per = (num_pages + kPlanThreads - 1) / kPlanThreads;
-  const int lo = min(static_cast<int64_t>(threadIdx.x) * per, static_cast<int64_t>(num_pages)), hi = min(lo + per, num_pages);
+  // in 64 bits: pools may have up to 2^31 - 1 pages
+  const int64_t pages = num_pages, per = (pages + kPlanThreads - 1) / kPlanThreads, begin = threadIdx.x * per;
+  const int lo = static_cast<int>(min(begin, pages)), hi = static_cast<int>(min(begin + per, pages));
   int mine = 0, live, moves;
   for (int i = lo; i < hi; ++i) mine += page_map[i];
   block_sum_upto(mine, s_warp, &live);

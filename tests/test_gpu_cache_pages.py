@@ -195,3 +195,22 @@ def test_pools_beyond_32_bits():
     assert r.block_tables.tolist() == [[2, 0, 1, -1, 3]] and r.counts.tolist() == [4, 3]
     assert all(torch.equal(pool[i], page(x)) for i, x in ((0, 4), (1, 3), (2, 2), (3, 1)))
     ops.check_status()
+
+
+def test_the_largest_pool():
+    """2^31 - 1 pages of a byte: the last run of the plan ends at the last page."""
+    from llm_from_scratch_b200 import ops
+    n = 2 ** 31 - 1
+    pool = torch.zeros(n, dtype=torch.uint8, device="cuda")
+    used = [n - 1, 3, n - 2, n - 1500, 2 ** 30 + 7, n - 3000000, 0]
+    for i, page in enumerate(used):
+        pool[page] = i + 1
+    tables = torch.tensor(used + [-1], dtype=torch.int32, device="cuda").view(2, 4)
+    r = ops.compact_pages(ops.PagePools([pool]), tables)
+    assert r.counts.tolist() == [7, 5]
+    want = {0: 0, 3: 3, 2 ** 30 + 7: 1, n - 3000000: 2, n - 1500: 4, n - 2: 5, n - 1: 6}
+    assert r.block_tables.flatten().tolist() == [want[p] for p in used] + [-1]
+    assert pool[:8].tolist() == [7, 5, 6, 2, 4, 3, 1, 0]
+    assert r.page_map[torch.tensor(used, device="cuda")].tolist() == [want[p] for p in used]
+    assert sum(int((part >= 0).sum()) for part in r.page_map.split(1 << 28)) == 7
+    ops.check_status()
