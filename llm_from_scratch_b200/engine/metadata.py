@@ -71,9 +71,11 @@ class StepParts:
 
 
 def block_table_array(s: Sequence) -> np.ndarray:
-    """int32 copy of ``s.block_table`` kept on the sequence between steps.  The block manager only ever
-    appends to the list or replaces it by a new list (deallocate), so the copy is extended by the new
-    entries when the list object is the same and rebuilt when it is not."""
+    """int32 copy of ``s.block_table`` kept on the sequence between steps.  The block manager appends to the
+    list or replaces it by a new list (deallocate), so the copy is extended by the new entries when the list
+    object is the same and rebuilt when it is not.  Entries of blocks that are given back (``release``) become
+    -1 in the list alone: the copy keeps their old ids, which may name blocks of others by now.  No kernel
+    reads them, as the model's attention sees nothing of these blocks any more."""
     bt = s.block_table
     n = len(bt)
     c = s._bt_cache
@@ -233,8 +235,9 @@ class DecodeBatchBuilder:
 
     With ``device_rows`` > 0 the builder also mirrors what the device-resident table holds at every batch
     position (which sequence row, at which epoch, how many entries), and ``build(..., patches=)`` emits only
-    the (position, column, block id) triples the device lacks: block tables are append-only between two
-    prefills of a sequence, so a steady batch costs one triple per sequence every ``block_size`` steps
+    the (position, column, block id) triples the device lacks: between two prefills of a sequence its block
+    table is appended to, and entries of blocks given back, whose old ids stay in both mirrors, are read by
+    nobody, so a steady batch costs one triple per sequence every ``block_size`` steps
     instead of a ``batch x max_blocks`` upload (the reference re-uploads the table, model_runner.py:263-268)."""
 
     def __init__(self, block_size: int, max_blocks: int, rows: int = 1024, device_rows: int = 0):
