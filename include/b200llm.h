@@ -833,7 +833,8 @@ int b200_window_decode(const void* q, const void* k_cache, const void* v_cache, 
  * the shortest run from the front whose weights reach top_p of their sum, at least one token; min_p (<= 0: off, at most 1) of
  * those the ones with w_i >= min_p; the draw is the first kept token, by number, at which the running sum of kept weights exceeds
  * u times their sum.  T <= 0 and rows without a logit above -inf: the first of the highest logits.  NaN counts as -inf.  The filter
- * arrays may be NULL (off).  vocab_size <= 2^24. */
+ * arrays may be NULL (off).  vocab_size <= 2^24.  Weights are whole numbers of 2^-S of the highest one, rounded to the nearest, with S = 45
+ * up to 131,072 tokens and a bit less for every doubling beyond; sums of them are exact. */
 size_t b200_sample_filtered_workspace_bytes(int64_t num_rows, int32_t vocab_size);
 int b200_sample_filtered(const void* logits, int64_t row_stride, int64_t num_rows, int32_t vocab_size, const float* uniforms,
                          const float* temperatures, const int32_t* top_k, const float* top_p, const float* min_p,
@@ -851,7 +852,8 @@ int b200_copy_pages(const int64_t* pools, const int64_t* page_bytes, int64_t lar
 /* Moves the pages that block_tables [rows, width] names (negative entries name none) to the front of all pools: with L of them, those
  * with an id >= L go, in ascending order, to the unnamed ids < L, in ascending order; nothing else is written in the pools.
  * out_tables [rows, width] = the tables with the new ids, page_map [num_pages] = new id or -1, counts = {L, moves}; source and target
- * [num_pages] receive the moves.  Entries outside the pool are reported and become -1. */
+ * [num_pages] receive the moves.  Entries outside the pool are reported and become -1.  For callers that keep ids in these tables alone: a
+ * b200_pool_create handle knows nothing of the moves. */
 int b200_compact_pages(const int64_t* pools, const int64_t* page_bytes, int64_t largest_page, int32_t num_pools, int64_t num_pages,
                        const int32_t* block_tables, int64_t bt_stride, int64_t rows, int32_t width, int32_t* out_tables,
                        int32_t* page_map, int32_t* source, int32_t* target, int32_t* counts, int32_t* status, void* stream);

@@ -7,8 +7,8 @@
 // Compaction: with L pages in use (named in a block table), the pages in use from id L on move, in ascending order, to the unused ids
 // below L, in ascending order.  What moves is never a target and the old places keep their contents, so all copies may run at once.
 //
-// Bound by the bytes: every page is read and written once (a compaction that moves 1,000 pages of 32 KB in
-// 16 pools, 1.06 GB: 166 us, 6.4 TB/s).  A CTA copies 32 KB of a page, all loads of a thread ahead of its stores; the CTAs of
+// Bound by the bytes: every page is read and written once (a compaction that moves 975 pages of 32 KB in
+// 16 pools, 1.02 GB: 166 us, 6.2 TB/s).  A CTA copies 32 KB of a page, all loads of a thread ahead of its stores; the CTAs of
 // a pool start before those of the next, so that a page which goes to several targets is mostly read from L2 after the first time.
 #include "common.cuh"
 

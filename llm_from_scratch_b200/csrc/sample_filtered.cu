@@ -17,9 +17,10 @@
 // found by sums over the threads' runs.  Many long rows go through sample_wide.cu.  Histograms hold a weight in three parts of 16 bits or more,
 // each a 32-bit counter: shared memory adds 32 bits at a time.
 //
-// Bound by the reads for large rows in principle; in fact by the weights (ten 64-bit operations each), the histogram's additions and the cluster's
-// barriers: a row of 32,000 under all filters 16 us, 64 rows 25 us (the first kernel, a CTA per row that read the logits for every byte of
-// a border: 199 and 270).
+// Bound by the reads for large rows in principle; in fact by latency, a chain of short steps with barriers between them: a row of 32,000 under
+// all filters 16.5 us, 64 rows 25 us (means of 20; the first kernel, a CTA per row that read the logits for every byte of a border: 199 and 270).
+// No unit is busy: 33 % of the issue slots at 64 rows.  Of the stalls there 19 % are for instructions, 17 % at barriers of the CTA, 14 % fixed
+// latency, 9 % at fences; of one row's 49 % for instructions and 15 % at barriers.
 #include <cooperative_groups.h>
 
 #include "sampling.cuh"
@@ -82,7 +83,7 @@ struct Row {
   RowShared* sh;
   float* own;                        // the thread's logits
   RowShape shape;
-  int rank, ranks, begin, mine;      // place in the cluster, first token of the CTA and of the thread
+  int rank, ranks, mine;             // place in the cluster, first token of the thread
   int S, turn;                       // turn of `parts`: two uses in a row do not meet, and a third comes behind a barrier
   float top, temperature, step, reach;
   double max, factor, floor_w;
@@ -115,8 +116,7 @@ struct Row {
   }
 };
 
-// A row's kernel runs through most of its code once, so fetching instructions sets the pace of small rows: of the stalls of one row of 32,000 more
-// than half are for instructions.  Calls out of line do not help, as they put the row's values into memory (256 rows of 131,072: 435 us
+// A row's kernel runs through most of its code once, so a row that is alone waits for instructions above all (see the top).  Calls out of line do not help, as they put the row's values into memory (256 rows of 131,072: 435 us
 // against 341).
 
 // Running sum over the CTA's threads, inclusive, and the CTA's sum.
@@ -425,7 +425,7 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, const int row, u
   w.shape = row_shape(V, ranks);
   const RowShape shape = w.shape;
   const int begin = rank * shape.slice;
-  w.begin = begin, w.mine = begin + tid * shape.run, w.own = data + tid * shape.stride;
+  w.mine = begin + tid * shape.run, w.own = data + tid * shape.stride;
   w.S = a.bits, w.turn = 0;
   w.edge = -INFINITY, w.edge_token = 0x7fffffff;
   w.temperature = fminf(a.temperatures[row], 1e30f);     // beyond that all finite logits weigh the same
@@ -624,8 +624,8 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, const int row, u
     if (nucleus) {
       // One standard deviation of the sum in front, and one of p times the whole, which in part is the same sum: with the bins' own widths a border
       // is seldom outside.  Such a row, and one whose bracket has more tokens than the list takes, finds it by the histograms of weights.  Means of
-      // 20 calls (us) at 3.5, 2, 1.2 and 0.6 deviations: 64 rows of 32,000, all filters, 28.8, 26.6, 25.6, 24.7; 256 with top-p 69, 63, 61, 59.  64 of
-      // bf16 with top-p: 25.4 (with the bins' middles and half a bin for each token as the bound: 48 .. 65)
+      // 20 calls (us) at 3.5, 2, 1.2, 1 and 0.6 deviations: 64 rows of 32,000, all filters, 28.4, 26.4, 25.2, 24.9, 24.5; 256 with top-p 68, 63, 60, 60,
+      // 58.  64 of bf16 with top-p: 25.3, 25.3, 25.2, 25.3, 24.8 (with the bins' middles and half a bin for each token as the bound: 48 .. 65)
       auto off = [&](float m, float e) {
         float root;
         asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(root) : "f"(e));

@@ -8,8 +8,8 @@
 //   draw     a CTA per row: the list in order, the borders, the 1,024 tokens in which the draw falls, the token
 //
 // The form in shared memory reads the logits once but passes six barriers of a cluster, with two CTAs on an SM to fill the waits: 256 rows of
-// 131,072 take it 251 us.  Here they are read three times and nothing waits inside a pass: 142 us (top 25, count 33, bracket 9, sum 71, draw 17,
-// the others 4; a read alone takes 21).  Bound by the weights of the sum: ten 64-bit operations for a token that has one, of which an SM
+// 131,072 take it 251 us.  Here they are read three times and nothing waits inside a pass: 141 us, mean of 20 (a read alone takes 21).  Launched
+// one by one with cold caches, which takes 152 in all: top 27, count 34, bracket 9, sum 69, draw 13.  Bound by the weights of the sum: ten 64-bit operations for a token that has one, of which an SM
 // does few at a time.  In bf16 140 .. 150 us (with the bins' middles for where their tokens lie the lists overflow and rows go to the other form: 280).
 // Rows that this form does not take (greedy ones, infinite logits, u <= 0, lists that overflow, a bracket that does not hold the border) are
 // named in a list, and the other form's kernel runs over that list at the end.
@@ -218,7 +218,7 @@ __global__ void __launch_bounds__(kRowThreads) wide_bracket_kernel(const Wide w)
       variance *= g * g * (1.f / (kPerUnit * kPerUnit));
       return g;
     };
-    // 1.2 standard deviations (as there): a border outside costs its row the other form (75 us), as does a bracket of more tokens than the list
+    // 1.2 standard deviations (the other form takes one, where a border outside costs less): a border outside costs its row the other form (75 us), as does a bracket of more tokens than the list
     // takes.  Means of 20 calls of 256 rows of 131,072, p up to 0.99: 142 us; with two 147, with 3.5 159
     auto off = [&](float m, float e) {
       float root;

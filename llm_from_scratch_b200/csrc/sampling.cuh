@@ -52,7 +52,7 @@ __device__ const double kTable[64] = {
     1.8340080864093424, 1.8539791250833855, 1.8741676341103, 1.8945759815869656,
     1.9152065613971474, 1.9360617934922943, 1.9571441241754002, 1.978456026387951};
 
-// The weight in units of 2^-S: 2^(n / 64) 2^(r / 64) with |r| <= 1/2, the second factor by its series up to r^4 (error 4e-14).
+// The weight in units of 2^-S by reduction to a table and a short series: 2^(n / 64) 2^(r / 64) with |r| <= 1/2, the second factor by its series up to r^4 (error 4e-14).
 // For logits no further from the maximum than 600 T.
 __device__ __forceinline__ double weight_within(float x, double max, double factor, int S, const double* table) {
   const double y = (static_cast<double>(x) - max) * factor;

@@ -29,7 +29,9 @@
 // Boxes whose keys no row of the CTA sees are not read: their coordinate lies behind the pool, where a copy delivers zeros.  What is
 // left are keys that some rows see and others do not.  Their scores become -inf in the other rows, but a weight of 0 would still turn an
 // infinity or NaN of the value row into a NaN: tiles in which some row is cut are searched for one, and a CTA that finds one
-// computes all its rows again, key by key, at its end.  The same way it leaves out keys of pages outside the pool.
+// computes all its rows again, key by key, at its end.  The same way it leaves out keys of pages outside the pool.  That costs: the portions
+// above with NaN behind the ends of 20 of the contexts, where pools that were not filled can hold some, take 10.7 ms instead of 45 us (the 32
+// tokens of a CTA times 4 heads read their keys one by one).  The engine's pools start as zeros.
 #include <cuda.h>
 
 #include "umma.cuh"

@@ -1664,7 +1664,8 @@ def window_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     q: [tokens, Hq, D], token stride free, portions at the ends of contexts of ``cu_seqlens_k`` lengths; caches
     [num_blocks, block_size, Hkv, D] (value heads may have a size of their own); ``block_tables`` [num_seqs, maxb] int32, of which only
     the entries of pages with a visible key count.  Rows that see no key are zeros; rows behind the last sequence are left as they
-    are (``out``).  Returns [tokens, Hq, Dv]."""
+    are (``out``).  Rows of the pools that no query sees may hold anything, but bf16 prompts are much slower where an infinity or NaN lies
+    among the values of a page beside rows that one sees: pools are best filled once before their first use.  Returns [tokens, Hq, Dv]."""
     dev = _cuda(q, k_cache, v_cache, block_tables, cu_seqlens_q, cu_seqlens_k, out)
     _on_current(dev)
     entries = cu_seqlens_q.numel()
@@ -1707,7 +1708,8 @@ def sample_filtered(logits: torch.Tensor, uniforms: torch.Tensor, temperatures: 
                     top_p: torch.Tensor | None = None, min_p: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
     """One token per row of ``logits`` [B, V] under temperature, top-k, top-p and min-p, drawn with ``uniforms`` [B] in [0, 1)
     (``b200_sample_filtered``).  Filters are per row: ``top_k`` int32 (<= 0 or >= V: off), ``top_p`` fp32 (>= 1: off), ``min_p`` fp32
-    (<= 0: off), None for all rows off; rows with a temperature <= 0 are greedy.  Equal logits count in the order of their tokens, and the
+    (<= 0: off), None for all rows off; rows with a temperature <= 0 are greedy.  Weights are held as whole numbers of 2^-45 of the highest
+    one (up to 131,072 tokens; a bit less for every doubling beyond), so those below half of that are not drawn.  Equal logits count in the order of their tokens, and the
     draw is the same for every launch: the same row and random number always give the same token.  Returns int64 [B]."""
     dev = _cuda(logits, uniforms, temperatures, top_k, top_p, min_p, out)
     _on_current(dev)
@@ -1798,7 +1800,8 @@ def compact_pages(pools: PagePools, block_tables: torch.Tensor) -> CompactedPage
     """Moves the pages that ``block_tables`` [rows, width] int32 names (negative entries name none; several entries may name one) to the
     front of all pools (``b200_compact_pages``): with L of them, those from id L on go, in ascending order, to the free ids below L, in
     ascending order.  The tables given are left as they are and the moved pages' old places keep their contents; no host wait.  Sequences
-    go on with the tables returned."""
+    go on with the tables returned.  For callers with pools and tables of their own: an engine's block manager keeps page ids in its free
+    list, its hashes and its sequences, and nothing renames them there."""
     dev = _cuda(pools.tensors[0], block_tables)
     _on_current(dev)
     if block_tables.dtype != torch.int32 or block_tables.dim() != 2 or (block_tables.shape[1] > 1 and block_tables.stride(1) != 1):
