@@ -416,7 +416,7 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, const int row, u
   float* data = reinterpret_cast<float*>(smem + sizeof(RowShared));
   // The other CTAs' shared memory may be written once they have all started: they say so here, the wait is in front of the first write.  No data
   // passes with it, so it orders nothing (relaxed).
-  asm volatile("barrier.cluster.arrive.relaxed.aligned;");
+  asm volatile("barrier.cluster.arrive.relaxed;");
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, V = a.vocab;
   Row w;
   w.sh = &sh;
@@ -489,7 +489,7 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, const int row, u
     for (int j = tid; j < kSteps; j += kRowThreads) sh.hist[j] = 0;
     if (tid == 0) sh.list_size = 0;
   }
-  asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait;" ::: "memory");
   w.top = key_value(combine_max(w, order_key(top)));
   if (!(w.temperature > 0.f) || w.top == -INFINITY) {
     const int token = first_highest(w, V);
