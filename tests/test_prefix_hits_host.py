@@ -1,8 +1,9 @@
 """Prefix hits of both block managers, followed by the contents of the pages: every key that a step reads belongs to the sequence that reads
-it, with blocks given back behind a window, forks, preemption and recomputed last blocks, in pools that evict all the time."""
+it, and the tables that captured decode steps keep on the device name the same pages, with blocks given back behind a window, forks, preemption and recomputed last blocks, in pools that evict all the time."""
 import itertools
 import random
 
+import numpy as np
 import pytest
 
 BS = 4
@@ -18,7 +19,10 @@ class Trace:
         self.s = Scheduler(max_num_sequences=16, max_num_batched_tokens=max_tokens, max_cached_blocks=blocks, block_size=BS, eos=-1, native_pool=native)
         self.s.attention_cut = cut
         self.window, self.first = cut or (1 << 30, 0)
+        from llm_from_scratch_b200.engine.metadata import DecodeBatchBuilder
         self.pages = {}
+        self.builder = DecodeBatchBuilder(BS, 128, rows=8, device_rows=16)      # what captured decode steps take their tables from
+        self.device = np.full((16, 128), -9, dtype=np.int32)
         self.log = []                       # what was scheduled, to compare two managers
 
     def add(self, tokens, n):
@@ -44,15 +48,33 @@ class Trace:
                     assert table[j // BS] >= 0 and self.pages.get((table[j // BS], j % BS)) == tuple(tokens[:j + 1]), \
                         f"the token at {p} reads a key at {j} that is not its own"
 
+    def _device_tables(self, batch):
+        """The table on the device, kept up by patches, names the pages of all that a decode step sees."""
+        ids, slots, lens, tables = (np.zeros(s, dtype=d) for s, d in ((16, np.int64), (16, np.int64), (16, np.int64), ((16, 128), np.int32)))
+        patches = np.zeros((24, 3), dtype=np.int32)
+        count = self.builder.build(batch, ids, slots, lens, tables, patches=patches)
+        if count < 0:
+            self.device[:len(batch)] = tables[:len(batch)]
+        for pos, col, block in patches[:max(count, 0)]:
+            self.device[pos, col] = block
+        for i, x in enumerate(batch):
+            p = x.num_tokens - 1
+            assert slots[i] == x.block_table[p // BS] * BS + p % BS and lens[i] == p + 1
+            for b in {j // BS for j in range(p + 1) if p - j < self.window or j < self.first}:
+                assert self.device[i, b] == x.block_table[b]
+
     def step(self, token, steps=1):
         batch, prefill = self.s.schedule()
         self.log.append((prefill, [(x.seq_id, list(x.block_table), x.num_cached_tokens) for x in batch]))
         k = 1 if prefill else self.s.plan_decode_window(batch, steps, 10 ** 6)
         rows, tokens = [], [list(x.token_ids) for x in batch]
         if prefill:                         # every layer writes the keys of all prompts before it reads any
+            self.builder.invalidate(batch)
             for x, t in zip(batch, tokens):
                 for p in range(x.num_cached_tokens, x.num_tokens):
                     self.pages[x.block_table[p // BS], p % BS] = tuple(t[:p + 1])
+        elif batch:
+            self._device_tables(batch)
         for _ in range(k):
             for x, t in zip(batch, tokens):
                 self._compute(t, x.block_table, x.num_cached_tokens if prefill else len(t) - 1, len(t))
